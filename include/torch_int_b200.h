@@ -256,6 +256,76 @@ int ti_attention_prefill_s8(const int8_t* q, int64_t ld_q, int64_t q_batch_strid
                             int64_t ctx_batch_stride, int64_t batch, int64_t heads, int64_t head_dim, int64_t T,
                             int64_t S, float alpha_qk, float alpha_pv, void* stream);
 
+/* ---- paged int8 key/value cache ----
+ *
+ * Pools of fixed-size pages, k_pages and v_pages int8 [num_pages, kv_heads, page_size, head_dim], instead of one
+ * rectangular tensor per layer: sequences of a batch may have any lengths, memory is handed out a page at a time.
+ * Sequence b of `batch` brings the new tokens [query_starts[b], query_starts[b + 1]) of `tokens` and holds
+ * kv_lens[b] keys, the new ones INCLUDED; its new token t sits at position kv_lens[b] - new tokens + t, and
+ * position p lies in page block_table[b * table_stride + p / page_size], row p % page_size.  query_starts
+ * [batch + 1], kv_lens [batch] and block_table are int32 DEVICE memory: a call has no host parameters that change
+ * with the lengths, only bounds, and can be captured in a CUDA graph.  max_query_len bounds a sequence's new tokens.
+ * head_dim 64, 80 or 128; page_size 16, 32, 64, 128 or 256; pools 16-byte aligned.
+ *
+ * A sequence whose lengths disagree with `tokens`, the bounds or the width of the block table is skipped (nothing
+ * of it is read or written) and sets the status word of ti_device_status to 211; a block table entry outside the
+ * pool sets it to 212 (its tokens are not stored; an attention that meets it reads page 0 instead). */
+typedef struct ti_paged_batch {
+  int8_t* k_pages;
+  int8_t* v_pages;
+  const int32_t* block_table;
+  const int32_t* query_starts;
+  const int32_t* kv_lens;
+  int64_t num_pages, kv_heads, page_size, head_dim;
+  int64_t table_stride, table_width; /* elements between rows of the block table, entries a row holds */
+  int64_t batch, tokens, max_query_len;
+} ti_paged_batch;
+
+/* Rotates, quantises and stores the new tokens' keys and values (and rotates and quantises their queries):
+ *   y1 = x1 * c - x2 * s,  y2 = x2 * c + x1 * s    over pairs of the first rotary_dim columns of q and k
+ *   int8 = sat_rne(alpha * y)                      every product and sum rounded to fp32; NaN gives 0
+ * with c = rotary[p * rotary_dim + i], s = rotary[p * rotary_dim + rotary_dim / 2 + i] of the token's position p.
+ * Pair i is columns (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`.  rotary NULL: no rotation.
+ * dtype of q, k and v: 0 fp32, 1 fp16, 2 bf16, 3 int8.  Token t of k starts at k + t * ld_k elements, heads and
+ * columns packed (q and v likewise; column blocks of a fused projection can be passed).  q NULL: no queries;
+ * otherwise q_out int8 [tokens, q_heads, head_dim].  rotary_dim a multiple of 16; all rows 16-byte aligned. */
+typedef struct ti_paged_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t ld_q, ld_k, ld_v;
+  int64_t q_heads;
+  const float* rotary;
+  int64_t rotary_rows, rotary_dim;
+  int8_t* q_out;
+  float q_alpha, k_alpha, v_alpha;
+  int32_t dtype, interleaved;
+} ti_paged_append_args;
+int ti_paged_append(const ti_paged_batch* batch, const ti_paged_append_args* args, void* stream);
+
+/* Causal attention of the new tokens over the paged cache, from one token per sequence to whole prompts:
+ *   s_j = alpha_qk * float(q . k_j) over the keys at positions j <= the token's,
+ *   ctx = alpha_pv * sum_j softmax(s)_j * v_j     -> out [tokens, q_heads, head_dim], rounded once
+ * Query head h reads key head h / (q_heads / kv_heads).  Unlike ti_attention_prefill_s8 and
+ * ti_decode_attention_s8 the probabilities are not rounded to int8.  A token that sees no key (fewer keys than
+ * new tokens) gives 0.  q int8, tokens ld_q elements apart; out_kind: 1 fp16, 2 bf16, 3 int8 (sat_rne).
+ * max_kv_len bounds kv_lens.  `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
+ * contents irrelevant, not shared by calls that may overlap on the GPU. */
+typedef struct ti_paged_attention_args {
+  const int8_t* q;
+  int64_t ld_q, q_heads, max_kv_len;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  float alpha_qk, alpha_pv;
+  int32_t out_kind;
+} ti_paged_attention_args;
+int ti_paged_attention(const ti_paged_batch* batch, const ti_paged_attention_args* args, void* stream);
+
+/* Bytes of workspace ti_paged_attention needs for these sizes (0: none). */
+int64_t ti_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t max_query_len, int64_t max_kv_len);
+
 /* ---- status ---- */
 
 /* Message of the last error raised on the calling thread ("" if none). */

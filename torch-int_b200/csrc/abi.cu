@@ -6,6 +6,7 @@
 #include "attention_prefill.h"
 #include "gemm_i8.h"
 #include "norm_quant.h"
+#include "paged.h"
 
 using namespace ti;
 
@@ -58,6 +59,25 @@ int bmm(const int8_t* A, const int8_t* B, void* C, int64_t batch, int64_t M, int
   g.alpha = alpha;
   g.epilogue = epi;
   return launch_gemm_i8(g, static_cast<cudaStream_t>(stream));
+}
+
+PagedBatch paged_batch(const ti_paged_batch& d) {
+  PagedBatch b;
+  b.k_pages = d.k_pages;
+  b.v_pages = d.v_pages;
+  b.block_table = d.block_table;
+  b.query_starts = d.query_starts;
+  b.kv_lens = d.kv_lens;
+  b.num_pages = d.num_pages;
+  b.kv_heads = d.kv_heads;
+  b.page_size = d.page_size;
+  b.head_dim = d.head_dim;
+  b.table_ld = d.table_stride;
+  b.table_width = d.table_width;
+  b.batch = d.batch;
+  b.tokens = d.tokens;
+  b.max_query_len = d.max_query_len;
+  return b;
 }
 
 }  // namespace
@@ -231,6 +251,55 @@ int ti_attention_prefill_s8(const int8_t* q, int64_t ld_q, int64_t q_batch_strid
   a.alpha_qk = alpha_qk;
   a.alpha_pv = alpha_pv;
   return attention_prefill_s8(a, static_cast<cudaStream_t>(stream));
+}
+
+int ti_paged_append(const ti_paged_batch* batch, const ti_paged_append_args* d, void* stream) {
+  if (batch == nullptr || d == nullptr) {
+    set_error("ti_paged_append: null descriptor");
+    return TI_E_INVALID;
+  }
+  PagedAppend a;
+  a.q = d->q;
+  a.k = d->k;
+  a.v = d->v;
+  a.dtype = d->dtype;
+  a.ld_q = d->ld_q;
+  a.ld_k = d->ld_k;
+  a.ld_v = d->ld_v;
+  a.q_heads = d->q_heads;
+  a.q_alpha = d->q_alpha;
+  a.k_alpha = d->k_alpha;
+  a.v_alpha = d->v_alpha;
+  a.rotary = d->rotary;
+  a.rotary_rows = d->rotary_rows;
+  a.rotary_dim = d->rotary_dim;
+  a.interleaved = d->interleaved;
+  a.q_out = d->q_out;
+  return paged_append(paged_batch(*batch), a, static_cast<cudaStream_t>(stream));
+}
+
+int ti_paged_attention(const ti_paged_batch* batch, const ti_paged_attention_args* d, void* stream) {
+  if (batch == nullptr || d == nullptr) {
+    set_error("ti_paged_attention: null descriptor");
+    return TI_E_INVALID;
+  }
+  PagedAttention a;
+  a.q = d->q;
+  a.ld_q = d->ld_q;
+  a.q_heads = d->q_heads;
+  a.max_kv_len = d->max_kv_len;
+  a.alpha_qk = d->alpha_qk;
+  a.alpha_pv = d->alpha_pv;
+  a.out = d->out;
+  a.out_kind = d->out_kind;
+  a.workspace = d->workspace;
+  a.workspace_bytes = d->workspace_bytes;
+  return paged_attention(paged_batch(*batch), a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t ti_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t max_query_len, int64_t max_kv_len) {
+  return paged_attention_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, max_query_len, max_kv_len);
 }
 
 const char* ti_last_error(void) { return last_error(); }

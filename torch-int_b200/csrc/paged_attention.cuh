@@ -1,0 +1,63 @@
+// What the kernels of attention over a paged cache share: parameters, the division of the keys, the store.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged_device.cuh"
+
+namespace ti {
+
+struct PagedAttnParams {
+  PagedView view;
+  const int8_t* q;
+  long long ld_q;
+  int q_heads, group;
+  int max_kv_len;
+  float scale_log2;   // alpha_qk * log2(e): scores are kept in the log2 domain
+  float alpha_pv;
+  void* out;
+  int out_kind;       // 1 fp16, 2 bf16, 3 int8
+  int row_tiles;      // of the largest sequence
+  int chunk;          // keys of a split, a multiple of 16
+  int max_splits;
+  int rows_below;     // sequences with more rows belong to the tile kernel (0: none do)
+  float* part_o;      // [tokens * q_heads][max_splits][head_dim], unnormalised
+  float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
+};
+
+struct PagedSplits {
+  int keys;  // keys visible to some row of the tile
+  int n;     // splits they are divided into, at least one
+};
+__device__ __forceinline__ PagedSplits paged_splits(int keys, int chunk) {
+  PagedSplits s;
+  s.keys = max(keys, 0);
+  s.n = max(1, (s.keys + chunk - 1) / chunk);
+  return s;
+}
+
+// Four neighbouring context values times `scale`, rounded once to the output type.
+__device__ __forceinline__ void paged_store4(const PagedAttnParams& p, long long at, float4 x, float scale) {
+  x.x *= scale;
+  x.y *= scale;
+  x.z *= scale;
+  x.w *= scale;
+  if (p.out_kind == 3) {
+    uint32_t lo, w;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(x.w)), "r"(__float2int_rn(x.z)));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(lo));
+    *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.out) + at) = w;
+  } else if (p.out_kind == 2) {
+    const __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
+  } else {
+    const __half2 u = __floats2half2_rn(x.x, x.y), w = __floats2half2_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
+  }
+}
+
+}  // namespace ti

@@ -30,7 +30,7 @@ __all__ = [
     "bmm_s8t_s8n_s8t", "bmm_s8t_s8n_f32t", "bmm_s8t_s8n_s32t", "dq_add_layernorm_q",
     # extras
     "layernorm_q", "softmax_q", "dq_add_layernorm_q_bias", "gemm_i8_ex", "transpose_values", "device_status",
-    "library_path",
+    "library_path", "paged_append", "paged_attention",
 ]
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libtorch_int_b200.so")
@@ -66,6 +66,32 @@ class _GemmDesc(ctypes.Structure):
         ("scatter_rows", _i64), ("scatter_ptrs", _ptr * 8),
         ("alpha_vec", _ptr), ("beta_vec", _ptr),
         ("workspace", _ptr), ("workspace_bytes", _i64), ("splits", ctypes.c_int32),
+    ]
+
+
+class _PagedBatch(ctypes.Structure):
+    # struct ti_paged_batch
+    _fields_ = [
+        ("k_pages", _ptr), ("v_pages", _ptr), ("block_table", _ptr), ("query_starts", _ptr), ("kv_lens", _ptr),
+        ("num_pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64),
+        ("table_stride", _i64), ("table_width", _i64), ("batch", _i64), ("tokens", _i64), ("max_query_len", _i64),
+    ]
+
+
+class _PagedAppendArgs(ctypes.Structure):
+    # struct ti_paged_append_args
+    _fields_ = [
+        ("q", _ptr), ("k", _ptr), ("v", _ptr), ("ld_q", _i64), ("ld_k", _i64), ("ld_v", _i64), ("q_heads", _i64),
+        ("rotary", _ptr), ("rotary_rows", _i64), ("rotary_dim", _i64), ("q_out", _ptr),
+        ("q_alpha", _f32), ("k_alpha", _f32), ("v_alpha", _f32), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+    ]
+
+
+class _PagedAttentionArgs(ctypes.Structure):
+    # struct ti_paged_attention_args
+    _fields_ = [
+        ("q", _ptr), ("ld_q", _i64), ("q_heads", _i64), ("max_kv_len", _i64), ("out", _ptr), ("workspace", _ptr),
+        ("workspace_bytes", _i64), ("alpha_qk", _f32), ("alpha_pv", _f32), ("out_kind", ctypes.c_int32),
     ]
 
 
@@ -108,6 +134,9 @@ _c_attention_prefill = _sig("ti_attention_prefill_s8",
                             [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64,
                              _i64, _i64, _i64, _i64, _i64, _f32, _f32, _ptr])
 _c_transpose_values = _sig("ti_transpose_values", [_ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr])
+_c_paged_append = _sig("ti_paged_append", [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_PagedAppendArgs), _ptr])
+_c_paged_attention = _sig("ti_paged_attention", [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_PagedAttentionArgs), _ptr])
+_c_paged_workspace = _sig("ti_paged_attention_workspace_bytes", [_i64] * 7, _i64)
 _c_last_error = _sig("ti_last_error", [], ctypes.c_char_p)
 _c_device_status = _sig("ti_device_status", [ctypes.POINTER(ctypes.c_int), _i32])
 _c_abi_version = _sig("ti_abi_version", [])
@@ -611,6 +640,126 @@ def transpose_values(v, vt, col0=0):
                                  _stream_ptr(v.device))
     _check(rc)
     return vt
+
+
+def _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, tokens, max_query_len):
+    """Checks the cache and the index tensors of a ragged batch; returns (descriptor, device, kv_heads, head_dim)."""
+    if not (isinstance(k_pages, torch.Tensor) and isinstance(v_pages, torch.Tensor) and k_pages.is_cuda
+            and k_pages.dtype == torch.int8 and v_pages.dtype == torch.int8 and k_pages.dim() == 4
+            and k_pages.shape == v_pages.shape and k_pages.device == v_pages.device
+            and k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise RuntimeError("k_pages and v_pages must be contiguous CUDA int8 tensors of the same shape "
+                           "[pages, kv_heads, page_size, head_dim]")
+    pages, hkv, page_size, d = k_pages.shape
+    dev = k_pages.device
+    for t, name in ((block_table, "block_table"), (query_starts, "query_starts"), (kv_lens, "kv_lens")):
+        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == dev):
+            raise RuntimeError(f"{name} must be an int32 tensor on {dev}")
+    if block_table.dim() != 2 or query_starts.dim() != 1 or kv_lens.dim() != 1 \
+            or query_starts.shape[0] != kv_lens.shape[0] + 1 or block_table.shape[0] != kv_lens.shape[0]:
+        raise RuntimeError(f"block_table {tuple(block_table.shape)}, query_starts {tuple(query_starts.shape)} and kv_lens "
+                           f"{tuple(kv_lens.shape)} must be [B, pages], [B + 1] and [B]")
+    batch, width = block_table.shape
+    if width > 1 and block_table.stride(1) != 1 or batch > 1 and block_table.stride(0) < width \
+            or not query_starts.is_contiguous() or not kv_lens.is_contiguous():
+        raise RuntimeError("block_table rows, query_starts and kv_lens must be packed")
+    if max_query_len is None:
+        max_query_len = tokens
+    stride = block_table.stride(0) if batch > 1 else width
+    return _PagedBatch(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(),
+                       kv_lens.data_ptr(), pages, hkv, page_size, d, stride, width, batch, tokens,
+                       max_query_len), dev, hkv, d
+
+
+def _paged_rows(t, name, tokens, d, dev, dtype):
+    """Element stride between the tokens of `t` [tokens, heads, d], whose heads and columns are packed."""
+    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and t.device == dev and t.dtype == dtype):
+        raise RuntimeError(f"{name} must be a 3-dimensional {dtype} tensor on {dev}")
+    n, h, dd = t.shape
+    st = t.stride()
+    if n != tokens or dd != d or d > 1 and st[2] != 1 or h > 1 and st[1] != d:
+        raise RuntimeError(f"{name} must be [{tokens}, heads, {d}] with packed heads, got shape {tuple(t.shape)} "
+                           f"and strides {st}")
+    return st[0] if n > 1 else h * d
+
+
+_PAGED_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+
+
+def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, max_query_len=None, q=None,
+                 k_alpha=1.0, v_alpha=1.0, q_alpha=1.0, rotary=None, interleaved=False):
+    """Stores the keys and values of a ragged batch of new tokens in a paged int8 cache (ti_paged_append).
+    k, v [N, Hkv, D] and optionally q [N, Hq, D], all fp32, fp16, bf16 or int8 (views of a fused projection are
+    fine: heads and columns packed, any token stride); k_pages, v_pages int8 [pages, Hkv, page_size, D];
+    query_starts int32 [B + 1]: sequence b's tokens; kv_lens int32 [B]: its keys, the new ones included;
+    block_table int32 [B, >= pages of the longest]: its pages in order.  int8 = sat_rne(alpha * x) after rotating
+    the first columns of q and k by `rotary`, fp32 [positions, rotary_dim] (torch_int.functional.paged.rotary_table):
+    pairs are the two halves of those columns, or neighbours with `interleaved`.  max_query_len bounds the new tokens
+    of a sequence (default: N).  Returns the rotated int8 queries [N, Hq, D], or None without q.
+    Extends torch.cat((past, new)) of torch_int/models/opt.py:113-116."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _PAGED_DTYPES:
+        raise RuntimeError("k must be a 3-dimensional float32, float16, bfloat16 or int8 tensor")
+    n = k.shape[0]
+    batch, dev, hkv, d = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
+    ld_k = _paged_rows(k, "k", n, d, dev, k.dtype)
+    ld_v = _paged_rows(v, "v", n, d, dev, k.dtype)
+    if k.shape[1] != hkv or v.shape[1] != hkv:
+        raise RuntimeError(f"k has {k.shape[1]} and v {v.shape[1]} heads, the cache {hkv}")
+    q_ptr = out_ptr = rot_ptr = None
+    ld_q = hq = rows = rd = 0
+    out = None
+    if q is not None:
+        ld_q = _paged_rows(q, "q", n, d, dev, k.dtype)
+        hq = q.shape[1]
+        out = torch.empty((n, hq, d), dtype=torch.int8, device=dev)
+        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    if rotary is not None:
+        if not (isinstance(rotary, torch.Tensor) and rotary.dtype == torch.float32 and rotary.device == dev
+                and rotary.dim() == 2 and rotary.is_contiguous()):
+            raise RuntimeError(f"rotary must be a contiguous float32 tensor [positions, rotary_dim] on {dev}")
+        rows, rd = rotary.shape
+        rot_ptr = rotary.data_ptr()
+    args = _PagedAppendArgs(q_ptr, k.data_ptr(), v.data_ptr(), ld_q, ld_k, ld_v, hq, rot_ptr, rows, rd, out_ptr,
+                            q_alpha, k_alpha, v_alpha, _PAGED_DTYPES[k.dtype], 1 if interleaved else 0)
+    with _on_device(dev):
+        rc = _c_paged_append(batch, args, _stream_ptr(dev))
+    _check(rc)
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, *, alpha_qk, alpha_pv, max_query_len=None,
+                    max_kv_len=None, out=None, out_dtype=torch.int8):
+    """Causal attention of a ragged batch of new tokens over a paged int8 cache (ti_paged_attention), from one
+    token per sequence to whole prompts.  q int8 [N, Hq, D] (heads and columns packed, any token stride), Hq a
+    multiple of the cache's heads; cache and index tensors as in paged_append, the new tokens already stored.
+    ctx = alpha_pv * softmax(alpha_qk * q . k) . v, rounded once to `out_dtype` (int8, float16 or bfloat16) or to
+    `out`'s; a token that sees no key gives 0.  max_query_len and max_kv_len bound the lengths (default: N and
+    what the block table can hold); close bounds cut the work better.  Returns [N, Hq, D]; rows that belong to no
+    sequence are left as they were.
+    Replaces the attention core of torch_int/models/opt.py:131-181 for sequences of unequal lengths."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise RuntimeError("q must be a 3-dimensional int8 tensor")
+    n, hq, _ = q.shape
+    batch, dev, hkv, d = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
+    ld_q = _paged_rows(q, "q", n, d, dev, torch.int8)
+    if max_kv_len is None:
+        max_kv_len = batch.table_width * batch.page_size
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=out_dtype, device=dev)
+    elif not (isinstance(out, torch.Tensor) and out.device == dev and out.shape == q.shape and out.is_contiguous()):
+        raise RuntimeError(f"out must be a contiguous {tuple(q.shape)} tensor on {dev}")
+    kind = _PAGED_DTYPES.get(out.dtype, 0)
+    if kind == 0:
+        raise RuntimeError(f"the context must be int8, float16 or bfloat16, not {out.dtype}")
+    need = _c_paged_workspace(batch.batch, n, hq, hkv, d, batch.max_query_len, max_kv_len)
+    # scratch of this call alone: the allocator orders its reuse by stream, and a captured graph keeps its own
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    args = _PagedAttentionArgs(q.data_ptr(), ld_q, hq, max_kv_len, out.data_ptr(), ws.data_ptr() if need else None,
+                               need, alpha_qk, alpha_pv, kind)
+    with _on_device(dev):
+        rc = _c_paged_attention(batch, args, _stream_ptr(dev))
+    _check(rc)
+    return out
 
 
 def set_dependent_launch(on):
