@@ -80,10 +80,11 @@ void set_narrow_a(int on);
 
 // Tensor map (CUtensorMap, 128 bytes, passed as an opaque pointer so that this header needs no
 // driver API types) of a K-major int8 operand [batch2, batch, rows, K]: box = 128 bytes of K x
-// box_rows x 1 x 1, 128-byte swizzle, out-of-range elements read as zero.  A batch index of extent
+// box_rows x 1 x box_batch2, 128-byte swizzle, out-of-range elements read as zero.  A batch index of extent
 // 1 or stride 0 becomes a dimension of extent 1.  Returns false after set_error().
 bool make_operand_map(void* tensor_map, const int8_t* ptr, int64_t K, int64_t rows, int64_t batch,
-                      int64_t batch2, int64_t ld, int64_t stride, int64_t stride2, int box_rows);
+                      int64_t batch2, int64_t ld, int64_t stride, int64_t stride2, int box_rows,
+                      int box_batch2 = 1);
 
 // Status word set by kernels whose bounded waits gave up (0 = ok).
 int* status_word_ptr();

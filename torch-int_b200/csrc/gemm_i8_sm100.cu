@@ -694,7 +694,8 @@ EncodeTiledFn get_encode_fn() {
 // K-major int8 operand [batch2, batch, rows, K] -> 4-D tensor map with a
 // (128 bytes of K) x box_rows x 1 x 1 box, 128-byte swizzle, zero fill.
 bool make_operand_map(void* tensor_map, const int8_t* ptr, int64_t K, int64_t rows, int64_t batch,
-                      int64_t batch2, int64_t ld, int64_t stride, int64_t stride2, int box_rows) {
+                      int64_t batch2, int64_t ld, int64_t stride, int64_t stride2, int box_rows,
+                      int box_batch2) {
   CUtensorMap* map = static_cast<CUtensorMap*>(tensor_map);
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) {
@@ -715,7 +716,8 @@ bool make_operand_map(void* tensor_map, const int8_t* ptr, int64_t K, int64_t ro
                         static_cast<cuuint64_t>(batch), static_cast<cuuint64_t>(batch2)};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld), static_cast<cuuint64_t>(stride),
                            static_cast<cuuint64_t>(stride2)};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows), 1,
+                       static_cast<cuuint32_t>(box_batch2)};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(ptr), dims, strides,
                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

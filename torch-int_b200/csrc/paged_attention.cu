@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
   grid_dep_launch();
   if (!paged_sequence(v, b, p.max_kv_len, &s)) return;
   const int G = p.group, rows = s.T * G, r0 = rt * R;
-  if (r0 >= rows || (p.rows_below != 0 && rows > p.rows_below)) return;
+  if (r0 >= rows || rows > p.rows_below) return;
   const int past = s.L - s.T;
   const PagedSplits sp = paged_splits(past + (min(r0 + R, rows) - 1) / G + 1, p.chunk);
   if (split >= sp.n) return;
@@ -328,24 +328,22 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
 
 // One warp per (token, query head): joins the partial contexts of the row's splits, in order.
 template <int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParams p, int tile_rows, int big_rows,
-                                                            int big_chunk) {
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParams p, int few_rows, int many_rows,
+                                                            int many_chunk) {
   const PagedView& v = p.view;
   const int b = blockIdx.y, lane = threadIdx.x & 31;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5);  // (token, head) of the sequence
-  const int q0 = v.query_starts[b], T = v.query_starts[b + 1] - q0, L = v.kv_lens[b];
-  grid_dep_wait();
   PagedSeq s;
-  if (!paged_sequence(v, b, p.max_kv_len, &s)) return;
-  (void)q0;
+  const bool ok = paged_sequence(v, b, p.max_kv_len, &s);
+  grid_dep_wait();
   const int t = row / p.q_heads, head = row % p.q_heads;
-  if (t >= T) return;
+  if (!ok || t >= s.T) return;
   // the row tile this row belonged to decides how many keys, hence splits, were visited
-  const int G = p.group, rows = T * G;
-  const bool big = p.rows_below != 0 && rows > p.rows_below;
-  const int R = big ? big_rows : tile_rows;
+  const int G = p.group, rows = s.T * G;
+  const bool many = rows > p.rows_below;
+  const int R = many ? many_rows : few_rows;
   const int r = t * G + head % G;
-  const PagedSplits sp = paged_splits(L - T + (min((r / R + 1) * R, rows) - 1) / G + 1, big ? big_chunk : p.chunk);
+  const PagedSplits sp = paged_splits(s.L - s.T + (min((r / R + 1) * R, rows) - 1) / G + 1, many ? many_chunk : p.chunk);
   if (sp.n == 1) return;  // written by the attention kernel
   const long long at = static_cast<long long>(s.q0 + t) * p.q_heads + head;
   const float2* ml = p.part_ml + at * p.max_splits;
@@ -373,47 +371,75 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
 }
 
 constexpr int SMS = 148;
+constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
+constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
 
+// How a call is cut.  Sequences with at most `few` rows per key head are served by paged_rows_kernel, the others by
+// paged_tiles_kernel; a kernel is left out where the bounds show that no sequence needs it.
 struct Plan {
-  int nt;          // 8-row tiles of a rows CTA
-  int row_tiles;
-  int chunk, splits;
+  bool rows, tiles;
+  int few;
+  int nt, row_tiles, chunk, row_splits;  // rows kernel: 8-row tiles of a CTA, CTAs of a sequence, keys of a split
+  PagedTilePlan tile;
+  int splits;                            // the larger number of splits: stride of the partial results
 };
 
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+int64_t div_up(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
-// How the work is cut.  `chunk` keys per CTA: enough CTAs for about two rounds on all SMs when every sequence has
-// the maximum length, so that shorter ones still fill them, but not below 128 keys (a CTA's fixed costs) nor above
-// MAX_CHUNK.
-Plan make_plan(int64_t batch, int64_t group, int64_t kv_heads, int64_t max_query_len, int64_t max_kv_len) {
-  Plan pl;
+Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int64_t max_query_len, int64_t max_kv_len) {
+  Plan pl = {};
   const int64_t rows = max_query_len * group;
-  pl.nt = rows <= 8 ? 1 : 2;
-  pl.row_tiles = static_cast<int>((rows + 8 * pl.nt - 1) / (8 * pl.nt));
-  const int64_t units = batch * kv_heads * pl.row_tiles;
-  const int64_t want = SMS * (pl.nt == 1 ? 4 : 2) * 2;
-  const int64_t splits = units >= want ? 1 : (want + units - 1) / units;
-  int64_t chunk = round_up((max_kv_len + splits - 1) / splits, 16);
-  if (chunk < 128) chunk = 128;
-  if (chunk > MAX_CHUNK) chunk = MAX_CHUNK;
-  pl.chunk = static_cast<int>(chunk);
-  pl.splits = static_cast<int>((max_kv_len + chunk - 1) / chunk);
-  if (pl.splits < 1) pl.splits = 1;
+  pl.few = group > TILE_ROWS ? 0x7FFFFFFF : FEW_ROWS;
+  pl.tiles = rows > pl.few;
+  // the shortest sequence brings at least the tokens that the others cannot hold
+  const int64_t shortest = tokens - (batch - 1) * max_query_len;
+  pl.rows = !pl.tiles || shortest * group <= pl.few;
+  pl.splits = 1;
+  if (pl.rows) {
+    // Enough CTAs for about two rounds on all SMs when every sequence has the maximum length, so that shorter ones
+    // still fill them, but not below 128 keys (a CTA's fixed costs) nor above MAX_CHUNK.
+    const int64_t most = rows < pl.few ? rows : pl.few;
+    pl.nt = most <= 8 ? 1 : 2;
+    pl.row_tiles = static_cast<int>(div_up(most, 8 * pl.nt));
+    const int64_t units = batch * kv_heads * pl.row_tiles, want = SMS * (pl.nt == 1 ? 4 : 2) * 2;
+    int64_t chunk = round_up(div_up(max_kv_len, units >= want ? 1 : div_up(want, units)), 16);
+    chunk = chunk < 128 ? 128 : chunk > MAX_CHUNK ? MAX_CHUNK : chunk;
+    pl.chunk = static_cast<int>(chunk);
+    pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
+    pl.splits = pl.row_splits;
+  }
+  if (pl.tiles) {
+    pl.tile.tokens_per_tile = static_cast<int>(TILE_ROWS / group);
+    pl.tile.pairs = static_cast<int>(div_up(max_query_len, 2 * pl.tile.tokens_per_tile));
+    const int64_t units = batch * kv_heads * pl.tile.pairs;
+    int64_t chunk = round_up(div_up(max_kv_len, units >= SMS ? 1 : div_up(SMS, units)), 128);
+    if (chunk < 512) chunk = 512;
+    pl.tile.chunk = static_cast<int>(chunk);
+    pl.tile.splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
+    if (pl.tile.splits > pl.splits) pl.splits = pl.tile.splits;
+  }
   return pl;
 }
 
 template <int D>
 int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(b.kv_heads),
-                  static_cast<unsigned>(b.batch * pl.row_tiles));
-  if (pl.nt == 1)
-    paged_rows_kernel<D, 1><<<grid, ROWS_THREADS, 0, stream>>>(p);
-  else
-    paged_rows_kernel<D, 2><<<grid, ROWS_THREADS, 0, stream>>>(p);
+  if (pl.rows) {
+    const dim3 grid(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
+                    static_cast<unsigned>(b.batch * pl.row_tiles));
+    if (pl.nt == 1)
+      paged_rows_kernel<D, 1><<<grid, ROWS_THREADS, 0, stream>>>(p);
+    else
+      paged_rows_kernel<D, 2><<<grid, ROWS_THREADS, 0, stream>>>(p);
+  }
   cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && pl.tiles) {
+    const int rc = launch_paged_tiles(b, p, pl.tile, stream);
+    if (rc != TI_OK) return rc;
+  }
   if (e == cudaSuccess && pl.splits > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((b.max_query_len * p.q_heads + 3) / 4), static_cast<unsigned>(b.batch));
+    cfg.gridDim = dim3(static_cast<unsigned>(div_up(b.max_query_len * p.q_heads, 4)), static_cast<unsigned>(b.batch));
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -421,7 +447,7 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_combine_kernel<D>, p, 8 * pl.nt, 0, 0);
+    e = cudaLaunchKernelEx(&cfg, paged_combine_kernel<D>, p, 8 * pl.nt, 2 * pl.tile.tokens_per_tile * p.group, pl.tile.chunk);
   }
   if (e != cudaSuccess) {
     set_error("paged_attention launch failed: %s", cudaGetErrorString(e));
@@ -436,7 +462,7 @@ int64_t paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q
                                         int64_t head_dim, int64_t max_query_len, int64_t max_kv_len) {
   if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_query_len <= 0 || max_kv_len <= 0) return 0;
   if (max_query_len > tokens) max_query_len = tokens;
-  const Plan pl = make_plan(batch, q_heads / kv_heads, kv_heads, max_query_len, max_kv_len);
+  const Plan pl = make_plan(batch, tokens, q_heads / kv_heads, kv_heads, max_query_len, max_kv_len);
   return pl.splits == 1 ? 0 : tokens * q_heads * pl.splits * (head_dim * 4 + 8);
 }
 
@@ -469,8 +495,8 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
     return TI_E_INVALID;
   }
   const int64_t group = a.q_heads / b.kv_heads;
-  const Plan pl = make_plan(b.batch, group, b.kv_heads, b.max_query_len, a.max_kv_len);
-  if (b.batch * pl.row_tiles > 65535 || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
+  const Plan pl = make_plan(b.batch, b.tokens, group, b.kv_heads, b.max_query_len, a.max_kv_len);
+  if (b.batch * static_cast<int64_t>(pl.row_tiles) > 65535 || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
     set_error("paged_attention: batch %lld x %lld new tokens is too large for one call", (long long)b.batch,
               (long long)b.max_query_len);
     return TI_E_INVALID;
@@ -501,7 +527,8 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   p.row_tiles = pl.row_tiles;
   p.chunk = pl.chunk;
   p.max_splits = pl.splits;
-  p.rows_below = 0;
+  p.rows_below = pl.tiles ? pl.few : 0x7FFFFFFF;
+  if (!pl.rows) p.rows_below = 0;
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + b.tokens * a.q_heads * pl.splits * b.head_dim);
   switch (b.head_dim) {

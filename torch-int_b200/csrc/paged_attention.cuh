@@ -22,10 +22,19 @@ struct PagedAttnParams {
   int row_tiles;      // of the largest sequence
   int chunk;          // keys of a split, a multiple of 16
   int max_splits;
-  int rows_below;     // sequences with more rows belong to the tile kernel (0: none do)
+  int rows_below;     // sequences with at most this many rows belong to the rows kernel, the others to the tile kernel
   float* part_o;      // [tokens * q_heads][max_splits][head_dim], unnormalised
   float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
 };
+
+// How the tile kernel (paged_attention_sm100.cu) cuts the work.
+struct PagedTilePlan {
+  int tokens_per_tile;  // of 128 rows: 128 / group
+  int pairs;            // pairs of row tiles of the largest sequence
+  int chunk;            // keys of a split, a multiple of 128
+  int splits;
+};
+int launch_paged_tiles(const PagedBatch& b, const PagedAttnParams& p, const PagedTilePlan& plan, cudaStream_t stream);
 
 struct PagedSplits {
   int keys;  // keys visible to some row of the tile

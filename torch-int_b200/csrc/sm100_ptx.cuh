@@ -315,6 +315,35 @@ __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// 32 registers per thread -> 32 columns of the thread's TMEM lane.
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem], f16 x f16 -> f32, issued by ONE thread.  A: one row per TMEM lane, two K
+// elements per 32-bit column.
+__device__ __forceinline__ void umma_f16_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // -------------------------------------------------------------- descriptors
 // Shared-memory matrix descriptor for a K-major tile whose rows are 128 B
 // wide and stored with the 128-byte swizzle (what a TMA load with
@@ -339,6 +368,28 @@ __host__ __device__ constexpr uint32_t make_idesc_s8s8s32(int mma_m, int mma_n) 
          | (0u << 15) | (0u << 16)                   // A, B K-major
          | (static_cast<uint32_t>(mma_n >> 3) << 17)  // N / 8
          | (static_cast<uint32_t>(mma_m >> 4) << 24); // M / 16
+}
+
+// Shared-memory matrix descriptor of a 16-bit operand whose M / N index is contiguous (MN-major), with the
+// 128-byte swizzle: 8 rows of K, 64 elements (128 B) each, make a 1024-byte atom; atoms follow one another
+// along K every 1024 B (SBO) and along M / N every `mn_stride` bytes (LBO).
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_addr, uint32_t mn_stride) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(mn_stride >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// Instruction descriptor for kind::f16 with fp16 operands, fp32 accumulator, A K-major, B MN-major.
+__host__ __device__ constexpr uint32_t make_idesc_f16_b_mn(int mma_m, int mma_n) {
+  return (1u << 4)                                    // D format: F32
+         | (0u << 7) | (0u << 10)                     // A, B format: F16
+         | (0u << 15) | (1u << 16)                    // A K-major, B MN-major
+         | (static_cast<uint32_t>(mma_n >> 3) << 17)
+         | (static_cast<uint32_t>(mma_m >> 4) << 24);
 }
 
 }  // namespace ti
