@@ -370,7 +370,6 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
   if (mine) paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
 }
 
-constexpr int SMS = 148;
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
 constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
 
@@ -402,7 +401,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     const int64_t most = rows < pl.few ? rows : pl.few;
     pl.nt = most <= 8 ? 1 : 2;
     pl.row_tiles = static_cast<int>(div_up(most, 8 * pl.nt));
-    const int64_t units = batch * kv_heads * pl.row_tiles, want = SMS * (pl.nt == 1 ? 4 : 2) * 2;
+    const int64_t units = batch * kv_heads * pl.row_tiles, want = PAGED_SMS * (pl.nt == 1 ? 4 : 2) * 2;
     int64_t chunk = round_up(div_up(max_kv_len, units >= want ? 1 : div_up(want, units)), 16);
     chunk = chunk < 128 ? 128 : chunk > MAX_CHUNK ? MAX_CHUNK : chunk;
     pl.chunk = static_cast<int>(chunk);
@@ -413,7 +412,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     pl.tile.tokens_per_tile = static_cast<int>(TILE_ROWS / group);
     pl.tile.pairs = static_cast<int>(div_up(max_query_len, 2 * pl.tile.tokens_per_tile));
     const int64_t units = batch * kv_heads * pl.tile.pairs;
-    int64_t chunk = round_up(div_up(max_kv_len, units >= SMS ? 1 : div_up(SMS, units)), 128);
+    int64_t chunk = round_up(div_up(max_kv_len, units >= PAGED_SMS ? 1 : div_up(PAGED_SMS, units)), 128);
     if (chunk < 512) chunk = 512;
     pl.tile.chunk = static_cast<int>(chunk);
     pl.tile.splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);

@@ -27,6 +27,8 @@ struct PagedAttnParams {
   float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
 };
 
+constexpr int PAGED_SMS = 148;
+
 // How the tile kernel (paged_attention_sm100.cu) cuts the work.
 struct PagedTilePlan {
   int tokens_per_tile;  // of 128 rows: 128 / group
@@ -67,6 +69,40 @@ __device__ __forceinline__ void paged_store4(const PagedAttnParams& p, long long
     *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
   }
+}
+
+// Eight neighbouring context values (fp32 bits) times `scale`, rounded once to the output type.
+__device__ __forceinline__ void paged_store8(const PagedAttnParams& p, long long at, const uint32_t (&o)[8], float scale) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(o[i]) * scale;
+  if (p.out_kind == 3) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t lo;
+      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(x[4 * i + 3])), "r"(__float2int_rn(x[4 * i + 2])));
+      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;"
+          : "=r"(w[i]) : "r"(__float2int_rn(x[4 * i + 1])), "r"(__float2int_rn(x[4 * i])), "r"(lo));
+    }
+    *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.out) + at) = make_uint2(w[0], w[1]);
+    return;
+  }
+  uint32_t w[4];
+  if (p.out_kind == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 u = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&u);
+    }
+  }
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace ti

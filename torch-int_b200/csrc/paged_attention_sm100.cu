@@ -11,19 +11,26 @@
 //
 // Why this division: per 256 x 128 scores the exponentials take 2048 clocks of an SM (16 per clock), the two
 // products 512 + 1024 and everything the softmax threads issue about 1300 slots per scheduler, so the exponentials
-// must never wait: two row tiles alternate, the products of one run under the softmax of the other.
-//   warps 0-3, 4-7  softmax and epilogue of row tile 0, 1      184 registers
-//   warps 8-11      int8 -> fp16 conversion of V               104
-//   warp 12, 13     TMA producer, MMA issuer                    40
+// must never wait.  S is one buffer of TMEM that both row tiles use in turn: a thread copies its row to registers
+// and hands S back, so the products of one tile run under the softmax of the other, and neither product is on the
+// path from one tile's exponentials to the next.  TMEM: S 128 columns, P 2 x 64, O 2 x 128.
+//   warps 0-7, 8-15  softmax and epilogue of row tile 0, 1: two threads per row, 64 keys each     96 registers
+//   warps 16-19      int8 -> fp16 conversion of V                                                  48
+//   warps 20-22      TMA producer, issuer of the scores, issuer of the contexts                    48
+// Two threads per row, not one: with one the chain from the scores to P (load 400 clocks, exponents and maximum 700,
+// exponentials 1400, store 200) was longer than the 2048 clocks it had to stay under; four warps per scheduler
+// overlap their chains.  The two threads agree on `off` through a barrier of their two warps that also carries the
+// vote; they exchange maxima only where off is raised.
+// The two products have an issuing thread each: one thread for both was the slowest part of the pipeline (a product
+// of 128 x 128 takes 64 clocks and about 100 to issue and commit).
+// The grid is persistent (one CTA per SM): copies and products of the next work item start while the last one's
+// context is still being written.
 // The score is formed without a conversion instruction: the bits of 1.5 * 2^23 + acc are acc + constant (|acc| <=
 // 2^21), and one fused multiply-add with off = c * (1.5 * 2^23 + max) - 7 gives the exponent; whatever off was
 // rounded to, it is the same for the whole row and cancels in the division by the sum.  off is raised only when an
 // exponent passes 15 (p <= 2^15 fits fp16 and, against the maximum's 2^7 or more, keeps weights down to 2^-31);
 // then O in TMEM is rescaled by the row's thread.  p is rounded to fp16 (2^-11) for the product, the row sum uses
-// it unrounded in fp32.
-//
-// S(j+1) of a row tile overwrites P(j) in TMEM: it is issued only after the commit of P(j) . V(j) has arrived.
-// Every wait is bounded (2 s) and reports through the status word.
+// it unrounded in fp32.  Every wait is bounded (2 s) and reports through the status word.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -42,20 +49,25 @@ constexpr int TILE_BYTES = TILE * 128;    // an int8 tile: 128 rows of 128 bytes
 constexpr int NK = 3;                     // stages of K
 constexpr int NV = 2;                     // stages of V as int8
 constexpr int NH = 2;                     // stages of V as fp16
-constexpr int THREADS = 512;
+constexpr int NQ = 2;                     // stages of the queries of a work item
+constexpr int MAX_SEQS = 512;             // sequences of a launch
+constexpr int THREADS = 768;
 constexpr int TMEM_COLS = 512;
-constexpr int REGS_SOFTMAX = 184, REGS_CONVERT = 104, REGS_OTHER = 40;  // per thread, of 512 x 128 at launch
-constexpr uint32_t TMEM_S = 0, TMEM_O = 256;  // + 128 * row tile
+constexpr int REGS_SOFTMAX = 96, REGS_CONVERT = 48, REGS_OTHER = 48;  // per thread, of 768 x 80 at launch
+constexpr uint32_t TMEM_S = 0, TMEM_P = 128, TMEM_O = 256;  // P + 64, O + 128 for row tile 1
 
 template <int D>
 struct Smem {
   static constexpr int HALF_BYTES = ((D + 63) / 64) * TILE_BYTES;  // fp16 V: 64 columns x 128 keys per 16 KB
   static constexpr int Q = 0;
-  static constexpr int K = Q + 2 * TILE_BYTES;
+  static constexpr int K = Q + NQ * 2 * TILE_BYTES;
   static constexpr int V = K + NK * TILE_BYTES;
   static constexpr int H = V + NV * TILE_BYTES;
-  static constexpr int BARS = H + NH * HALF_BYTES;
+  static constexpr int SEQ = H + NH * HALF_BYTES;
+  static constexpr int XCHG = SEQ + MAX_SEQS * 16;  // [row tile][half][row]: maxima, then sums
+  static constexpr int BARS = XCHG + 2 * 2 * 2 * TILE * 4;
   static constexpr int BYTES = 1024 + BARS + 512;
+  static_assert(BYTES <= 232448, "227 KB of shared memory");
 };
 
 enum : int {
@@ -70,16 +82,13 @@ enum : int {
   TI_ERR_PT_P_FULL = 229,    // MMA warp waited for probabilities
   TI_ERR_PT_PV = 230,        // MMA warp waited for a product with V
   TI_ERR_PT_O_FULL = 231,    // epilogue waited for the context
+  TI_ERR_PT_Q_EMPTY = 232,   // producer waited for a stage of the queries
+  TI_ERR_PT_S_EMPTY = 233,   // MMA warp waited for the scores to be read
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 // Two fp32 operations in one instruction.
@@ -113,62 +122,124 @@ __device__ __forceinline__ uint2 halves4(uint32_t w) {
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
+// Barrier of `threads` threads that returns whether any of them passed true.
+__device__ __forceinline__ bool barrier_or(int id, int threads, bool mine) {
+  int any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, %1, %2, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<int>(mine))
+      : "memory");
+  return any != 0;
+}
+
 struct TileParams {
   PagedAttnParams a;
   int tokens_per_tile;  // 128 / group
-  int pairs;            // row tile pairs of the largest sequence
   int chunk;            // keys of a split, a multiple of 128
+  int seq0, seqs;       // sequences of this launch
+};
+
+// Sequences of the launch in shared memory; `first` = work items (per key head) of the sequences before it.
+struct SeqInfo {
+  int q0, T, L, first;
+};
+
+// One work item: two row tiles of a sequence, one key head, one split of the keys.
+struct Item {
+  int b, h, split, t0, k0;
+  int n_splits;     // of this pair of row tiles
+  int nt0, nt1;     // key tiles of the two row tiles
+  int q0, T, L;
+};
+
+__device__ __forceinline__ int splits_of(int L, int chunk) { return max(1, (L + chunk - 1) / chunk); }
+
+// Work item `idx`: sequences in order, in each the row tiles that see most keys first, then splits, then heads.
+__device__ __forceinline__ Item item_at(const TileParams& tp, const SeqInfo* seq, int idx) {
+  Item w;
+  const int hkv = tp.a.view.kv_heads;
+  const int e = idx / hkv;
+  w.h = idx - e * hkv;
+  int lo = 0, hi = tp.seqs - 1;
+  while (lo < hi) {  // last sequence with first <= e
+    const int mid = (lo + hi + 1) >> 1;
+    if (seq[mid].first <= e) lo = mid;
+    else hi = mid - 1;
+  }
+  const SeqInfo s = seq[lo];
+  const int TPT = tp.tokens_per_tile, ns = splits_of(s.L, tp.chunk);
+  const int at = (e - s.first) / ns;
+  w.b = tp.seq0 + lo;
+  w.q0 = s.q0;
+  w.T = s.T;
+  w.L = s.L;
+  w.split = e - s.first - at * ns;
+  w.t0 = ((s.T + 2 * TPT - 1) / (2 * TPT) - 1 - at) * 2 * TPT;
+  w.k0 = w.split * tp.chunk;
+  const int past = s.L - s.T;
+  w.n_splits = paged_splits(past + min(w.t0 + 2 * TPT, s.T), tp.chunk).n;
+  const int end0 = min(w.k0 + tp.chunk, past + min(w.t0 + TPT, s.T));
+  const int end1 = min(w.k0 + tp.chunk, past + min(w.t0 + 2 * TPT, s.T));
+  w.nt0 = end0 > w.k0 ? (end0 - w.k0 + TILE - 1) / TILE : 0;
+  w.nt1 = w.t0 + TPT < s.T && end1 > w.k0 ? (end1 - w.k0 + TILE - 1) / TILE : 0;
+  return w;
+}
+
+// A ring position: stage and the parity of its current use.
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++stage == n) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
 };
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                   const __grid_constant__ CUtensorMap tmap_v, const TileParams tp) {
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ TileParams tp) {
   const PagedAttnParams& p = tp.a;
   const PagedView& v = p.view;
-  const int b = blockIdx.z, h = blockIdx.y;
-  // the last rows of a sequence see most keys: they go first
-  const int pair = tp.pairs - 1 - static_cast<int>(blockIdx.x) / p.max_splits, split = blockIdx.x % p.max_splits;
-  grid_dep_launch();
-  PagedSeq s;
-  if (!paged_sequence(v, b, p.max_kv_len, &s)) return;
-  const int G = p.group, TPT = tp.tokens_per_tile;
-  const int t0 = pair * 2 * TPT;
-  if (t0 >= s.T || s.T * G <= p.rows_below) return;
-  const int past = s.L - s.T;
-  const PagedSplits sp = paged_splits(past + min(t0 + 2 * TPT, s.T), tp.chunk);
-  if (split >= sp.n) return;
-  const int k0 = split * tp.chunk;
-  int nt[2];  // key tiles of the two row tiles
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const bool any = t0 + x * TPT < s.T;
-    const int end = min(k0 + tp.chunk, past + min(t0 + (x + 1) * TPT, s.T));
-    nt[x] = any && end > k0 ? (end - k0 + TILE - 1) / TILE : 0;
-  }
-  const int n_tiles = max(nt[0], nt[1]);
-
   using SM = Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  SeqInfo* seq = reinterpret_cast<SeqInfo*>(smem + SM::SEQ);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BARS);
   uint64_t* q_full = bars;
-  uint64_t* k_full = q_full + 1;
+  uint64_t* q_empty = q_full + NQ;
+  uint64_t* k_full = q_empty + NQ;
   uint64_t* k_empty = k_full + NK;
   uint64_t* v_full = k_empty + NK;
   uint64_t* v_empty = v_full + NV;
   uint64_t* h_full = v_empty + NV;
   uint64_t* h_empty = h_full + NH;
   uint64_t* s_full = h_empty + NH;
-  uint64_t* p_full = s_full + 2;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_empty + 1;
   uint64_t* pv_done = p_full + 2;
   uint64_t* o_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* warp_sum = reinterpret_cast<int*>(tmem_slot + 2);  // [24]
+  float* s_top = reinterpret_cast<float*>(smem + SM::XCHG);
+  float* s_sum = s_top + 2 * 2 * TILE;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dep_launch();
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(q_full), 1);
+    for (int i = 0; i < NQ; ++i) {
+      mbar_init(smem_u32(&q_full[i]), 1);
+      mbar_init(smem_u32(&q_empty[i]), 1);
+    }
     for (int i = 0; i < NK; ++i) {
       mbar_init(smem_u32(&k_full[i]), 1);
       mbar_init(smem_u32(&k_empty[i]), 1);
@@ -183,272 +254,379 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&s_full[x]), 1);
-      mbar_init(smem_u32(&p_full[x]), 128);
+      mbar_init(smem_u32(&p_full[x]), 256);
       mbar_init(smem_u32(&pv_done[x]), 1);
       mbar_init(smem_u32(&o_full[x]), 1);
     }
+    mbar_init(smem_u32(s_empty), 256);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
-  if (warp == 13) {
+  if (warp == 21) {
     tmem_alloc<1>(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish<1>();
+  }
+  // ---- the sequences of this launch: one per thread, work items counted by a prefix sum
+  int items;
+  {
+    PagedSeq s = {0, 0, 0};
+    int n = 0;
+    const int i = threadIdx.x;
+    if (i < tp.seqs && paged_sequence(v, tp.seq0 + i, p.max_kv_len, &s) && s.T * p.group > p.rows_below)
+      n = (s.T + 2 * tp.tokens_per_tile - 1) / (2 * tp.tokens_per_tile) * splits_of(s.L, tp.chunk);
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    int before = 0;
+    items = 0;
+    for (int k = 0; k < THREADS / 32; ++k) {
+      if (k < warp) before += warp_sum[k];
+      items += warp_sum[k];
+    }
+    items *= v.kv_heads;
+    if (i < MAX_SEQS) seq[i] = SeqInfo{s.q0, s.T, s.L, before + sum - n};
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int G = p.group, TPT = tp.tokens_per_tile;
+  const int first = blockIdx.x, step = gridDim.x;
 
-  if (warp >= 12) {
+  if (warp >= 20) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
-    if (warp == 12) {
+    if (warp == 20) {
       // ------------------------------------------------------------ TMA producer: one lane per page of a tile
       const int P = 1 << v.page_shift;
       const int box = min(P, TILE), boxes = TILE / box;  // a 256-key page holds two tiles
-      const int pages_used = (s.L + P - 1) >> v.page_shift;
-      auto page_at = [&](int j) {  // page of this lane's rows of tile j; one past the pool (zeros) behind the last key
-        const int i = (k0 + j * TILE + lane * box) >> v.page_shift;
-        if (lane >= boxes || i >= pages_used) return v.num_pages;
-        const int page = paged_page(v, b, i);
-        return page < 0 ? 0 : page;
-      };
-      if (lane == 0) {
-        const uint32_t rows = G * TPT;
-        const int tiles = (nt[0] > 0) + (nt[1] > 0);
-        mbar_expect_tx(smem_u32(q_full), tiles * rows * 128);
-        for (int x = 0; x < 2; ++x)
-          if (nt[x] > 0)
-            tma_load_4d(smem_u32(smem + SM::Q + x * TILE_BYTES), &tmap_q, smem_u32(q_full), 0, 0, h, s.q0 + t0 + x * TPT);
-      }
-      __syncwarp();
+      Ring rk, rv, rq;
       bool ok = true;
-      int next = page_at(0);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int page = next;
-        if (j + 1 < n_tiles) next = page_at(j + 1);
-        const int row = (k0 + j * TILE + lane * box) & (P - 1);
-        const int ks = j % NK, vs = j % NV;
-        ok = mbar_wait_status(smem_u32(&k_empty[ks]), ((j / NK) & 1) ^ 1, abort_flag, v.status, TI_ERR_PT_K_EMPTY);
+      for (int idx = first; idx < items && ok; idx += step) {
+        const Item w = item_at(tp, seq, idx);
+        const int n_tiles = max(w.nt0, w.nt1);
+        if (n_tiles == 0) continue;
+        const int pages_used = (w.L + P - 1) >> v.page_shift;
+        auto page_at = [&](int j) {  // page of this lane's rows of tile j; one past the pool (zeros) behind the last key
+          const int i = (w.k0 + j * TILE + lane * box) >> v.page_shift;
+          if (lane >= boxes || i >= pages_used) return v.num_pages;
+          const int page = paged_page(v, w.b, i);
+          return page < 0 ? 0 : page;
+        };
+        int next = page_at(0);
+        ok = mbar_wait_status(smem_u32(&q_empty[rq.stage]), rq.phase ^ 1, abort_flag, v.status, TI_ERR_PT_Q_EMPTY);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_expect_tx(smem_u32(&k_full[ks]), TILE_BYTES);
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&q_full[rq.stage]);
+          mbar_expect_tx(bar, ((w.nt0 > 0) + (w.nt1 > 0)) * G * TPT * 128);
+          const uint32_t dst = smem_u32(smem + SM::Q + rq.stage * 2 * TILE_BYTES);
+          if (w.nt0 > 0) tma_load_4d(dst, &tmap_q, bar, 0, 0, w.h, w.q0 + w.t0);
+          if (w.nt1 > 0) tma_load_4d(dst + TILE_BYTES, &tmap_q, bar, 0, 0, w.h, w.q0 + w.t0 + TPT);
+        }
         __syncwarp();
-        if (lane < boxes)
-          tma_load_4d(smem_u32(smem + SM::K + ks * TILE_BYTES + lane * box * 128), &tmap_k, smem_u32(&k_full[ks]), 0, row, h, page);
-        ok = mbar_wait_status(smem_u32(&v_empty[vs]), ((j / NV) & 1) ^ 1, abort_flag, v.status, TI_ERR_PT_V_EMPTY);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_expect_tx(smem_u32(&v_full[vs]), TILE_BYTES);
-        __syncwarp();
-        if (lane < boxes)
-          tma_load_4d(smem_u32(smem + SM::V + vs * TILE_BYTES + lane * box * 128), &tmap_v, smem_u32(&v_full[vs]), 0, row, h, page);
+        rq.next(NQ);
+        for (int j = 0; j < n_tiles; ++j) {
+          const int page = next;
+          if (j + 1 < n_tiles) next = page_at(j + 1);
+          const int row = (w.k0 + j * TILE + lane * box) & (P - 1);
+          ok = mbar_wait_status(smem_u32(&k_empty[rk.stage]), rk.phase ^ 1, abort_flag, v.status, TI_ERR_PT_K_EMPTY);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (lane == 0) mbar_expect_tx(smem_u32(&k_full[rk.stage]), TILE_BYTES);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_4d(smem_u32(smem + SM::K + rk.stage * TILE_BYTES + lane * box * 128), &tmap_k,
+                        smem_u32(&k_full[rk.stage]), 0, row, w.h, page);
+          rk.next(NK);
+          ok = mbar_wait_status(smem_u32(&v_empty[rv.stage]), rv.phase ^ 1, abort_flag, v.status, TI_ERR_PT_V_EMPTY);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (lane == 0) mbar_expect_tx(smem_u32(&v_full[rv.stage]), TILE_BYTES);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_4d(smem_u32(smem + SM::V + rv.stage * TILE_BYTES + lane * box * 128), &tmap_v,
+                        smem_u32(&v_full[rv.stage]), 0, row, w.h, page);
+          rv.next(NV);
+        }
+        ok = __all_sync(0xffffffffu, ok);
       }
-    } else if (warp == 13 && lane == 0) {
-      // ------------------------------------------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc_s = make_idesc_s8s8s32(TILE, TILE);
-      constexpr uint32_t idesc_o = make_idesc_f16_b_mn(TILE, D);
-      bool ok = n_tiles > 0 && mbar_wait_status(smem_u32(q_full), 0, abort_flag, v.status, TI_ERR_PT_Q);
-      auto scores = [&](int x, int j) {  // S_x = Q_x . K_j
-        const int ks = j % NK;
-        ok = mbar_wait_status(smem_u32(&k_full[ks]), (j / NK) & 1, abort_flag, v.status, TI_ERR_PT_K_FULL);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t dq = make_smem_desc_sw128(smem_u32(smem + SM::Q + x * TILE_BYTES));
-        const uint64_t dk = make_smem_desc_sw128(smem_u32(smem + SM::K + ks * TILE_BYTES));
+    } else if (warp == 21 && lane == 0) {
+      // ------------------------------------------------------------------------- issuer of the scores S = Q . K
+      constexpr uint32_t idesc = make_idesc_s8s8s32(TILE, TILE);
+      const uint64_t desc = make_smem_desc_sw128(0);
+      const uint32_t hi = static_cast<uint32_t>(desc >> 32), lo0 = static_cast<uint32_t>(desc);
+      const uint32_t q_lo = lo0 + (smem_u32(smem + SM::Q) >> 4), k_lo = lo0 + (smem_u32(smem + SM::K) >> 4);
+      Ring rq, rk;
+      bool ok = true;
+      uint32_t s_parity = 1;  // the first wait passes at once
+      for (int idx = first; idx < items && ok; idx += step) {
+        const Item w = item_at(tp, seq, idx);
+        const int n_tiles = max(w.nt0, w.nt1);
+        if (n_tiles == 0) continue;
+        ok = mbar_wait_status(smem_u32(&q_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_Q);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          ok = mbar_wait_status(smem_u32(&k_full[rk.stage]), rk.phase, abort_flag, v.status, TI_ERR_PT_K_FULL);
+          const uint32_t b_lo = k_lo + rk.stage * (TILE_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < (D + 31) / 32; ++k) umma_i8<1>(tmem + TMEM_S + x * TILE, dq + 2 * k, dk + 2 * k, idesc_s, k != 0);
-        umma_commit(smem_u32(&s_full[x]));
-        if (x == 1 || j >= nt[1]) umma_commit(smem_u32(&k_empty[ks]));  // the last row tile that reads K_j
-      };
-      for (int x = 0; x < 2 && ok; ++x)
-        if (nt[x] > 0) scores(x, 0);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int hs = j % NH;
-        ok = mbar_wait_status(smem_u32(&h_full[hs]), (j / NH) & 1, abort_flag, v.status, TI_ERR_PT_H_FULL);
-        const uint64_t dv = make_smem_desc_mn_sw128(smem_u32(smem + SM::H + hs * SM::HALF_BYTES), TILE_BYTES);
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (j >= nt[x]) continue;
-          ok = mbar_wait_status(smem_u32(&p_full[x]), j & 1, abort_flag, v.status, TI_ERR_PT_P_FULL);
-          if (!ok) break;
-          tc_fence_after();
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || j >= (x ? w.nt1 : w.nt0)) continue;
+            ok = mbar_wait_status(smem_u32(s_empty), s_parity, abort_flag, v.status, TI_ERR_PT_S_EMPTY);
+            if (!ok) continue;
+            s_parity ^= 1;
+            tc_fence_after();
+            const uint32_t a_lo = q_lo + (rq.stage * 2 + x) * (TILE_BYTES >> 4);
 #pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)
-            umma_f16_a_tmem(tmem + TMEM_O + x * TILE, tmem + TMEM_S + x * TILE + 8 * k, dv + k * (2048 >> 4), idesc_o,
-                            j != 0 || k != 0);
-          if (x == 1 || j >= nt[1]) umma_commit(smem_u32(&h_empty[hs]));
-          if (j + 1 < nt[x]) {
-            umma_commit(smem_u32(&pv_done[x]));
-            ok = mbar_wait_status(smem_u32(&pv_done[x]), j & 1, abort_flag, v.status, TI_ERR_PT_PV);
-            if (ok) scores(x, j + 1);
-          } else {
-            umma_commit(smem_u32(&o_full[x]));
+            for (int k = 0; k < (D + 31) / 32; ++k) umma_i8_lo(tmem + TMEM_S, a_lo + 2 * k, b_lo + 2 * k, hi, idesc, k != 0);
+            umma_commit(smem_u32(&s_full[x]));
           }
+          if (!ok) break;
+          umma_commit(smem_u32(&k_empty[rk.stage]));
+          rk.next(NK);
+        }
+        if (ok) umma_commit(smem_u32(&q_empty[rq.stage]));
+        rq.next(NQ);
+      }
+    } else if (warp == 22 && lane == 0) {
+      // -------------------------------------------------------------------- issuer of the contexts O += P . V
+      constexpr uint32_t idesc = make_idesc_f16_b_mn(TILE, D);
+      const uint64_t desc = make_smem_desc_mn_sw128(0, TILE_BYTES);
+      const uint32_t hi = static_cast<uint32_t>(desc >> 32);
+      const uint32_t v_lo = static_cast<uint32_t>(desc) + (smem_u32(smem + SM::H) >> 4);
+      Ring rh;
+      bool ok = true;
+      uint32_t p_phase[2] = {0, 0};
+      for (int idx = first; idx < items && ok; idx += step) {
+        const Item w = item_at(tp, seq, idx);
+        const int n_tiles = max(w.nt0, w.nt1);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          ok = mbar_wait_status(smem_u32(&h_full[rh.stage]), rh.phase, abort_flag, v.status, TI_ERR_PT_H_FULL);
+          const uint32_t b_lo = v_lo + rh.stage * (SM::HALF_BYTES >> 4);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int nt = x ? w.nt1 : w.nt0;
+            if (!ok || j >= nt) continue;
+            ok = mbar_wait_status(smem_u32(&p_full[x]), p_phase[x], abort_flag, v.status, TI_ERR_PT_P_FULL);
+            if (!ok) continue;
+            p_phase[x] ^= 1;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < TILE / 16; ++k)  // 16 keys of V are 2048 bytes
+              umma_f16_a_tmem(tmem + TMEM_O + x * TILE, tmem + TMEM_P + x * 64 + 8 * k, b_lo + k * (2048 >> 4), hi, idesc,
+                              j != 0 || k != 0);
+            umma_commit(smem_u32(j + 1 < nt ? &pv_done[x] : &o_full[x]));
+          }
+          if (!ok) break;
+          umma_commit(smem_u32(&h_empty[rh.stage]));
+          rh.next(NH);
         }
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 16) {
     // ------------------------------------------------------------------------------- conversion of V to fp16
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONVERT));
-    const int w = warp - 8;
+    const int wv = warp - 16;
     // A quarter warp takes four 16-byte chunks of the keys k and k ^ 5: with the swizzle (chunk ^ key % 8) their
     // 16-byte reads and writes fall into different banks.
     const int sub = lane >> 3, c = lane & 3;
     const int key8 = (lane >> 2) & 1 ? sub ^ 5 : sub;  // of a group of 8 keys
+    Ring rv, rh;
     bool ok = true;
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const int vs = j % NV, hs = j % NH;
-      ok = mbar_wait_status(smem_u32(&v_full[vs]), (j / NV) & 1, abort_flag, v.status, TI_ERR_PT_V_FULL);
-      if (!ok) break;
-      ok = mbar_wait_status(smem_u32(&h_empty[hs]), ((j / NH) & 1) ^ 1, abort_flag, v.status, TI_ERR_PT_H_EMPTY);
-      if (!ok) break;
-      const uint8_t* src = smem + SM::V + vs * TILE_BYTES;
-      uint8_t* dst = smem + SM::H + hs * SM::HALF_BYTES;
-      auto convert = [&](int key, int chunk) {
-        const uint4 in = *reinterpret_cast<const uint4*>(src + key * 128 + ((chunk ^ (key & 7)) << 4));
-        const uint2 h0 = halves4(in.x), h1 = halves4(in.y), h2 = halves4(in.z), h3 = halves4(in.w);
-        uint8_t* row = dst + (chunk >> 2) * TILE_BYTES + key * 128;
-        const int o = (chunk & 3) * 2;
-        *reinterpret_cast<uint4*>(row + ((o ^ (key & 7)) << 4)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
-        *reinterpret_cast<uint4*>(row + (((o + 1) ^ (key & 7)) << 4)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
-      };
+    for (int idx = first; idx < items && ok; idx += step) {
+      const Item w = item_at(tp, seq, idx);
+      const int n_tiles = max(w.nt0, w.nt1);
+      for (int j = 0; j < n_tiles; ++j) {
+        ok = mbar_wait_status(smem_u32(&v_full[rv.stage]), rv.phase, abort_flag, v.status, TI_ERR_PT_V_FULL);
+        if (ok) ok = mbar_wait_status(smem_u32(&h_empty[rh.stage]), rh.phase ^ 1, abort_flag, v.status, TI_ERR_PT_H_EMPTY);
+        if (!ok) break;
+        const uint8_t* src = smem + SM::V + rv.stage * TILE_BYTES;
+        uint8_t* dst = smem + SM::H + rh.stage * SM::HALF_BYTES;
+        auto convert = [&](int key, int chunk) {
+          const uint4 in = *reinterpret_cast<const uint4*>(src + key * 128 + ((chunk ^ (key & 7)) << 4));
+          const uint2 h0 = halves4(in.x), h1 = halves4(in.y), h2 = halves4(in.z), h3 = halves4(in.w);
+          uint8_t* row = dst + (chunk >> 2) * TILE_BYTES + key * 128;
+          const int o = (chunk & 3) * 2;
+          *reinterpret_cast<uint4*>(row + ((o ^ (key & 7)) << 4)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+          *reinterpret_cast<uint4*>(row + (((o + 1) ^ (key & 7)) << 4)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
+        };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = (w * 4 + i) * 8 + key8;
-        convert(key, c);
-        if (D == 128) convert(key, 4 + c);
+        for (int i = 0; i < 4; ++i) {
+          const int key = (wv * 4 + i) * 8 + key8;
+          convert(key, c);
+          if (D == 128) convert(key, 4 + c);
+        }
+        if (D == 80) convert(wv * 32 + lane, 4);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&h_full[rh.stage]));
+        mbar_arrive(smem_u32(&v_empty[rv.stage]));
+        rv.next(NV);
+        rh.next(NH);
       }
-      if (D == 80) convert(w * 32 + lane, 4);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(smem_u32(&h_full[hs]));
-      mbar_arrive(smem_u32(&v_empty[vs]));
     }
   } else {
     // ----------------------------------------------------------------------------------- softmax and epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    const int x = warp >> 2;                       // row tile
-    const int r = (warp & 3) * 32 + lane;          // row of it = TMEM lane
-    const int tile_t0 = t0 + x * TPT;
-    const int t = tile_t0 + r / G;
-    const bool valid = r < G * TPT && t < s.T;
-    const int lim = past + min(t, s.T - 1);        // last visible key
-    const int lim_min = past + tile_t0;
+    const int x = warp >> 3, half = (warp >> 2) & 1;   // row tile, 64 keys of a key tile
+    const int r = (warp & 3) * 32 + lane;              // row of the tile = TMEM lane
+    const int r_token = r / G, r_head = r - r_token * G;
+    const int pair_bar = 1 + x * 4 + (warp & 3);       // barrier of the two warps that share 32 rows
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + TMEM_S + x * TILE + lane_off, to = tmem + TMEM_O + x * TILE + lane_off;
-    constexpr uint32_t kMagic = 0x4B400000u;       // bits of 1.5 * 2^23
+    const uint32_t ts = tmem + TMEM_S + half * 64 + lane_off, tpp = tmem + TMEM_P + x * 64 + half * 32 + lane_off;
+    const uint32_t to = tmem + TMEM_O + x * TILE + half * (D / 2) + lane_off;  // this thread's columns of O
+    float* my_top = s_top + (x * 2 + half) * TILE + r;
+    const float* other_top = s_top + (x * 2 + (half ^ 1)) * TILE + r;
+    constexpr uint32_t kMagic = 0x4B400000u;           // bits of 1.5 * 2^23
     const float c = p.scale_log2;
-    const int tiles = nt[x];
-    float off = c * 12582912.f;
-    float l = 0.f;
+    uint32_t s_phase = 0, pv_phase = 0, o_phase = 0;
+    // A wait that gives up (all later ones then return at once) does not leave the loops: the barriers of two warps
+    // have no limit, so both warps pass every one of them and only the results are not stored.
     bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      ok = mbar_wait_status(smem_u32(&s_full[x]), j & 1, abort_flag, v.status, TI_ERR_PT_S_FULL);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      const int kt = k0 + j * TILE;
-      const bool edge = kt + TILE - 1 > lim_min;   // some row does not see all keys of the tile
-      uint32_t a[4][32];
-      auto exponents = [&]() {                     // a = exponent of every score, -inf where hidden
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld_32x32(ts + 32 * q, a[q]);
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+      if (!mbar_wait_status(smem_u32(bar), parity, abort_flag, v.status, code)) ok = false;
+      __syncwarp();
+    };
+    for (int idx = first; idx < items; idx += step) {
+      const Item w = item_at(tp, seq, idx);
+      const int tiles = x ? w.nt1 : w.nt0;
+      const int tile_t0 = w.t0 + x * TPT;
+      const int t = tile_t0 + r_token;
+      const int past = w.L - w.T;
+      const int lim = past + min(t, w.T - 1) - half * 64;  // last visible key, counted from this thread's columns
+      const int lim_min = past + tile_t0;
+      float off = c * 12582912.f;
+      float l = 0.f;
+      for (int j = 0; j < tiles; ++j) {
+        wait(&s_full[x], s_phase, TI_ERR_PT_S_FULL);
+        s_phase ^= 1;
+        tc_fence_after();
+        const int kt = w.k0 + j * TILE;
+        uint32_t a[2][32];                             // scores, then their exponents
+        tmem_ld_32x32(ts, a[0]);
+        tmem_ld_32x32(ts + 32, a[1]);
         tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(s_empty));
         const float2 cc = make_float2(c, c), oo = make_float2(-off, -off);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const float2 e = fma2(make_float2(__uint_as_float(a[q][i] + kMagic), __uint_as_float(a[q][i + 1] + kMagic)), cc, oo);
             a[q][i] = __float_as_uint(e.x);
             a[q][i + 1] = __float_as_uint(e.y);
           }
-        if (edge) {
+        if (kt + TILE - 1 > lim_min) {                 // some row does not see all keys of the tile
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (kt + 32 * q + i > lim) a[q][i] = 0xFF800000u;
         }
-      };
-      exponents();
-      float mx[4];
+        float mx[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mx[q] = __uint_as_float(a[q][0]);
+        for (int q = 0; q < 4; ++q) {
+          mx[q] = __uint_as_float(a[q >> 1][(q & 1) * 16]);
 #pragma unroll
-        for (int i = 1; i < 31; i += 2) mx[q] = max3(mx[q], __uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1]));
-        mx[q] = fmaxf(mx[q], __uint_as_float(a[q][31]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool raise = j == 0 || top > 15.f;
-      if (__any_sync(0xffffffffu, raise)) {
-        const float old = off;
-        if (raise && top > -INFINITY) off += top - 7.f;
-        const float corr = ex2(old - off);
-        l *= corr;
-        if (j > 0) {
-#pragma unroll
-          for (int q = 0; q < (D + 31) / 32; ++q) {  // columns beyond an 80-wide context hold nothing that is used
-            tmem_ld_32x32(to + 32 * q, a[0]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) a[0][i] = __float_as_uint(__uint_as_float(a[0][i]) * corr);
-            tmem_st_32x32(to + 32 * q, a[0]);
-          }
-          tmem_st_wait();
+          for (int i = 1; i < 16; ++i) mx[q] = fmaxf(mx[q], __uint_as_float(a[q >> 1][(q & 1) * 16 + i]));
         }
-        exponents();
-      }
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (barrier_or(pair_bar, 64, j == 0 || top > 15.f)) {
+          *my_top = top;
+          asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+          top = fmaxf(top, *other_top);
+          const float old = off;
+          if ((j == 0 || top > 15.f) && top > -INFINITY) off += top - 7.f;
+          const float by = old - off;
+          const float corr = ex2(by);
+          l *= corr;
+          const float2 by2 = make_float2(by, by);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+            for (int i = 0; i < 32; i += 2) {
+              const float2 e = add2(make_float2(__uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1])), by2);
+              a[q][i] = __float_as_uint(e.x);
+              a[q][i + 1] = __float_as_uint(e.y);
+            }
+          if (j > 0) {                                 // the product that last wrote O is done
+            wait(&pv_done[x], pv_phase, TI_ERR_PT_PV);
+            tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t o[8];
+              tmem_ld_32x8(to + 8 * q, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st_32x8(to + 8 * q, o);
+            }
+          }
+        }
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 e = make_float2(ex2(__uint_as_float(a[half * 2 + q][i])), ex2(__uint_as_float(a[half * 2 + q][i + 1])));
+            const float2 e = make_float2(ex2(__uint_as_float(a[q][i])), ex2(__uint_as_float(a[q][i + 1])));
             sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
-            pk[q * 16 + i / 2] = pack_half2(e.x, e.y);
+            pk[i / 2] = pack_half2(e.x, e.y);
           }
-        tmem_st_32x32(ts + 32 * half, pk);
+          if (q == 0 && j > 0) {                       // the product that last read P is done
+            wait(&pv_done[x], pv_phase, TI_ERR_PT_PV);
+            pv_phase ^= 1;
+            tc_fence_after();
+          }
+          tmem_st_32x16(tpp + 16 * q, pk);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_full[x]));
       }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(smem_u32(&p_full[x]));
-    }
-    if (ok && tiles > 0) ok = mbar_wait_status(smem_u32(&o_full[x]), 0, abort_flag, v.status, TI_ERR_PT_O_FULL);
-    if (__all_sync(0xffffffffu, ok) && tile_t0 < s.T) {
-      tc_fence_after();
-      const long long at = static_cast<long long>(s.q0 + t) * p.q_heads + h * G + r % G;
-      const bool whole = sp.n == 1;
+      if (tiles > 0) {
+        wait(&o_full[x], o_phase, TI_ERR_PT_O_FULL);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+      if (w.split >= w.n_splits) continue;             // beyond the keys of this pair of row tiles
+      s_sum[(x * 2 + half) * TILE + r] = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      l = s_sum[x * 2 * TILE + r] + s_sum[(x * 2 + 1) * TILE + r];
+      const bool valid = ok && r < G * TPT && t < w.T;
+      const long long at = static_cast<long long>(w.q0 + t) * p.q_heads + w.h * G + r_head;
+      const bool whole = w.n_splits == 1;
       const float scale = l > 0.f ? p.alpha_pv / l : 0.f;
-      float* po = p.part_o + (at * p.max_splits + split) * D;
-      if (valid && !whole) p.part_ml[at * p.max_splits + split] = make_float2(l > 0.f ? off : -1e30f, l);
-#pragma unroll
-      for (int q = 0; q < (D + 31) / 32; ++q) {
-        uint32_t a[32];
+      float* po = p.part_o + (at * p.max_splits + w.split) * D + half * (D / 2);
+      if (valid && !whole && half == 0) p.part_ml[at * p.max_splits + w.split] = make_float2(l > 0.f ? off : -1e30f, l);
+#pragma unroll 1
+      for (int q = 0; q < D / 16; ++q) {
+        uint32_t o[8];
         if (tiles > 0) {
-          tmem_ld_32x32(to + 32 * q, a);
+          tmem_ld_32x8(to + 8 * q, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) a[i] = 0;
+          for (int i = 0; i < 8; ++i) o[i] = 0;
         }
         if (valid) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            if (32 * q + i >= D) break;
-            const float4 y = make_float4(__uint_as_float(a[i]), __uint_as_float(a[i + 1]), __uint_as_float(a[i + 2]),
-                                         __uint_as_float(a[i + 3]));
-            if (whole)
-              paged_store4(p, at * D + 32 * q + i, y, scale);
-            else
-              *reinterpret_cast<float4*>(po + 32 * q + i) = y;
+          if (whole) {
+            paged_store8(p, at * D + half * (D / 2) + 8 * q, o, scale);
+          } else {
+            *reinterpret_cast<uint4*>(po + 8 * q) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(po + 8 * q + 4) = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         __syncwarp();
       }
+      // the next item's sums are written after its barriers, and its products overwrite O only after this thread's
+      // next arrival on p_full
+      tc_fence_before();
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
     }
   }
 
@@ -463,7 +641,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
   }
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 21) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, TMEM_COLS);
   }
@@ -474,7 +652,6 @@ int launch(const PagedBatch& b, const PagedAttnParams& a, const PagedTilePlan& p
   TileParams tp;
   tp.a = a;
   tp.tokens_per_tile = plan.tokens_per_tile;
-  tp.pairs = plan.pairs;
   tp.chunk = plan.chunk;
   CUtensorMap tq, tk, tv;
   const int64_t page_bytes = b.page_size * D;
@@ -491,14 +668,19 @@ int launch(const PagedBatch& b, const PagedAttnParams& a, const PagedTilePlan& p
       cudaFuncAttributes fa;
       return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : 0;
     }();
-    if (regs * THREADS < REGS_SOFTMAX * 256 + REGS_CONVERT * 128 + REGS_OTHER * 128) {
+    if (regs * THREADS < REGS_SOFTMAX * 512 + REGS_CONVERT * 128 + REGS_OTHER * 128) {
       set_error("paged_attention: the kernel was built with %d registers per thread, too few for its warpgroups", regs);
       return TI_E_CUDA;
     }
-    const dim3 grid(static_cast<unsigned>(plan.pairs * a.max_splits), static_cast<unsigned>(b.kv_heads),
-                    static_cast<unsigned>(b.batch));
-    kernel<<<grid, THREADS, Smem<D>::BYTES, stream>>>(tq, tk, tv, tp);
-    e = cudaGetLastError();
+    // persistent: one CTA per SM, or per work item where the bounds allow fewer
+    const int64_t most = (b.batch < MAX_SEQS ? b.batch : MAX_SEQS) * static_cast<int64_t>(plan.pairs) * plan.splits * b.kv_heads;
+    const unsigned grid = static_cast<unsigned>(most < PAGED_SMS ? most : PAGED_SMS);
+    for (int64_t b0 = 0; b0 < b.batch && e == cudaSuccess; b0 += MAX_SEQS) {
+      tp.seq0 = static_cast<int>(b0);
+      tp.seqs = static_cast<int>(b.batch - b0 < MAX_SEQS ? b.batch - b0 : MAX_SEQS);
+      kernel<<<grid, THREADS, Smem<D>::BYTES, stream>>>(tq, tk, tv, tp);
+      e = cudaGetLastError();
+    }
   }
   if (e != cudaSuccess) {
     set_error("paged_attention launch failed: %s", cudaGetErrorString(e));
