@@ -71,38 +71,41 @@ __device__ __forceinline__ void paged_store4(const PagedAttnParams& p, long long
   }
 }
 
-// Eight neighbouring context values (fp32 bits) times `scale`, rounded once to the output type.
-__device__ __forceinline__ void paged_store8(const PagedAttnParams& p, long long at, const uint32_t (&o)[8], float scale) {
-  float x[8];
+// Sixteen neighbouring context values (fp32 bits) as `width` 16-byte pieces: 4 as they are (a partial result), 2 and
+// 1 times `scale` and rounded once to fp16 / bf16 and int8.
+__device__ __forceinline__ void paged_convert16(int width, int out_kind, const uint32_t (&o)[16], float scale, uint4 (&piece)[4]) {
+  if (width == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(o[i]) * scale;
-  if (p.out_kind == 3) {
-    uint32_t w[2];
+    for (int i = 0; i < 4; ++i) piece[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    return;
+  }
+  float x[16];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(o[i]) * scale;
+  uint32_t w[8];
+  if (width == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       uint32_t lo;
       asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(x[4 * i + 3])), "r"(__float2int_rn(x[4 * i + 2])));
       asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;"
           : "=r"(w[i]) : "r"(__float2int_rn(x[4 * i + 1])), "r"(__float2int_rn(x[4 * i])), "r"(lo));
     }
-    *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.out) + at) = make_uint2(w[0], w[1]);
-    return;
-  }
-  uint32_t w[4];
-  if (p.out_kind == 2) {
+  } else if (out_kind == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&u);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const __half2 u = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&u);
     }
   }
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  piece[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (width == 2) piece[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 }  // namespace ti

@@ -54,7 +54,14 @@ constexpr int MAX_SEQS = 512;             // sequences of a launch
 constexpr int THREADS = 768;
 constexpr int TMEM_COLS = 512;
 constexpr int REGS_SOFTMAX = 96, REGS_CONVERT = 48, REGS_OTHER = 48;  // per thread, of 768 x 80 at launch
-constexpr uint32_t TMEM_S = 0, TMEM_P = 128, TMEM_O = 256;  // P + 64, O + 128 for row tile 1
+
+// Columns of TMEM: scores (64-wide heads leave room for a second buffer), P of both row tiles, O of both.
+template <int D>
+struct Tmem {
+  static constexpr int NS = D == 64 ? 2 : 1;
+  static constexpr uint32_t S = 0, P = NS * TILE, O = P + 2 * 64, O_STRIDE = D == 64 ? 64 : 128;
+  static_assert(O + 2 * O_STRIDE <= TMEM_COLS, "512 columns");
+};
 
 template <int D>
 struct Smem {
@@ -64,8 +71,9 @@ struct Smem {
   static constexpr int V = K + NK * TILE_BYTES;
   static constexpr int H = V + NV * TILE_BYTES;
   static constexpr int SEQ = H + NH * HALF_BYTES;
-  static constexpr int XCHG = SEQ + MAX_SEQS * 16;  // [row tile][half][row]: maxima, then sums
-  static constexpr int BARS = XCHG + 2 * 2 * 2 * TILE * 4;
+  static constexpr int XCHG = SEQ + MAX_SEQS * 20;  // [row tile][half][row]: maxima, then sums
+  static constexpr int ITEM = XCHG + 2 * 2 * 2 * TILE * 4;
+  static constexpr int BARS = ITEM + NQ * 48;
   static constexpr int BYTES = 1024 + BARS + 512;
   static_assert(BYTES <= 232448, "227 KB of shared memory");
 };
@@ -84,11 +92,36 @@ enum : int {
   TI_ERR_PT_O_FULL = 231,    // epilogue waited for the context
   TI_ERR_PT_Q_EMPTY = 232,   // producer waited for a stage of the queries
   TI_ERR_PT_S_EMPTY = 233,   // MMA warp waited for the scores to be read
+  TI_ERR_PT_ITEM = 234,      // a warp waited for the next work item
 };
+
+// Bounded wait (2 s), written for few instructions: the loops of the warps of a scheduler share an instruction cache
+// of about 12 KB, and misses in it were the largest stall of this kernel.
+__device__ __forceinline__ uint32_t timer_ns() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t t0 = timer_ns();
+#pragma unroll 1
+  do {
+    if (mbar_try_wait(bar, parity)) return true;
+  } while (*abort_flag == 0 && timer_ns() - t0 < static_cast<uint32_t>(TI_WAIT_LIMIT_NS));
+  *abort_flag = 1;
+  atomicCAS(status, 0, code);
+  return false;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 // Two fp32 operations in one instruction.
@@ -147,25 +180,46 @@ struct TileParams {
 
 // Sequences of the launch in shared memory; `first` = work items (per key head) of the sequences before it.
 struct SeqInfo {
-  int q0, T, L, first;
+  int q0, T, L, first, pairs;
 };
 
-// One work item: two row tiles of a sequence, one key head, one split of the keys.
-struct Item {
-  int b, h, split, t0, k0;
-  int n_splits;     // of this pair of row tiles
-  int nt0, nt1;     // key tiles of the two row tiles
+// One work item: two row tiles of a sequence, one key head, one split of the keys.  The TMA producer posts them in
+// shared memory, in the order of the stages of the queries, for all other warps.
+struct __align__(16) Item {
+  int nt0, nt1;     // key tiles of the two row tiles; nt0 < 0: no more items
   int q0, T, L;
+  int t0, k0;       // first token of the row tiles, first key of the split
+  int h, split, n_splits;
+  int b, unused;
 };
 
 __device__ __forceinline__ int splits_of(int L, int chunk) { return max(1, (L + chunk - 1) / chunk); }
 
-// Work item `idx`: sequences in order, in each the row tiles that see most keys first, then splits, then heads.
-__device__ __forceinline__ Item item_at(const TileParams& tp, const SeqInfo* seq, int idx) {
+// The work items of a CTA: every gridDim.x-th of (entry, key head), heads fastest; without a division per item.
+struct Walk {
+  int e, h, de, dh, hkv, entries;
+  __device__ __forceinline__ Walk(int kv_heads, int n_entries) : hkv(kv_heads), entries(n_entries) {
+    e = static_cast<int>(blockIdx.x) / hkv;
+    h = static_cast<int>(blockIdx.x) - e * hkv;
+    de = static_cast<int>(gridDim.x) / hkv;
+    dh = static_cast<int>(gridDim.x) - de * hkv;
+  }
+  __device__ __forceinline__ bool more() const { return e < entries; }
+  __device__ __forceinline__ void next() {
+    e += de;
+    h += dh;
+    if (h >= hkv) {
+      h -= hkv;
+      ++e;
+    }
+  }
+};
+
+// Entry e: sequences in order, in each the row tiles that see most keys first, then splits.
+__device__ __forceinline__ Item item_at(const TileParams& tp, const SeqInfo* seq, const Walk& walk) {
   Item w;
-  const int hkv = tp.a.view.kv_heads;
-  const int e = idx / hkv;
-  w.h = idx - e * hkv;
+  const int e = walk.e;
+  w.h = walk.h;
   int lo = 0, hi = tp.seqs - 1;
   while (lo < hi) {  // last sequence with first <= e
     const int mid = (lo + hi + 1) >> 1;
@@ -173,17 +227,18 @@ __device__ __forceinline__ Item item_at(const TileParams& tp, const SeqInfo* seq
     else hi = mid - 1;
   }
   const SeqInfo s = seq[lo];
-  const int TPT = tp.tokens_per_tile, ns = splits_of(s.L, tp.chunk);
-  const int at = (e - s.first) / ns;
+  const int TPT = tp.tokens_per_tile;
+  const int ns = s.L > tp.chunk ? splits_of(s.L, tp.chunk) : 1;
+  const int at = ns > 1 ? (e - s.first) / ns : e - s.first;
   w.b = tp.seq0 + lo;
   w.q0 = s.q0;
   w.T = s.T;
   w.L = s.L;
   w.split = e - s.first - at * ns;
-  w.t0 = ((s.T + 2 * TPT - 1) / (2 * TPT) - 1 - at) * 2 * TPT;
+  w.t0 = (s.pairs - 1 - at) * 2 * TPT;
   w.k0 = w.split * tp.chunk;
   const int past = s.L - s.T;
-  w.n_splits = paged_splits(past + min(w.t0 + 2 * TPT, s.T), tp.chunk).n;
+  w.n_splits = ns > 1 ? paged_splits(past + min(w.t0 + 2 * TPT, s.T), tp.chunk).n : 1;
   const int end0 = min(w.k0 + tp.chunk, past + min(w.t0 + TPT, s.T));
   const int end1 = min(w.k0 + tp.chunk, past + min(w.t0 + 2 * TPT, s.T));
   w.nt0 = end0 > w.k0 ? (end0 - w.k0 + TILE - 1) / TILE : 0;
@@ -210,21 +265,24 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const PagedAttnParams& p = tp.a;
   const PagedView& v = p.view;
   using SM = Smem<D>;
+  using TM = Tmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   SeqInfo* seq = reinterpret_cast<SeqInfo*>(smem + SM::SEQ);
+  volatile Item* item = reinterpret_cast<volatile Item*>(smem + SM::ITEM);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BARS);
   uint64_t* q_full = bars;
   uint64_t* q_empty = q_full + NQ;
-  uint64_t* k_full = q_empty + NQ;
+  uint64_t* i_full = q_empty + NQ;
+  uint64_t* k_full = i_full + NQ;
   uint64_t* k_empty = k_full + NK;
   uint64_t* v_full = k_empty + NK;
   uint64_t* v_empty = v_full + NV;
   uint64_t* h_full = v_empty + NV;
   uint64_t* h_empty = h_full + NH;
   uint64_t* s_full = h_empty + NH;
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_empty + 1;
+  uint64_t* s_empty = s_full + 4;  // s_full: [row tile][buffer], s_empty: [buffer]
+  uint64_t* p_full = s_empty + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* o_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
@@ -238,7 +296,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < NQ; ++i) {
       mbar_init(smem_u32(&q_full[i]), 1);
-      mbar_init(smem_u32(&q_empty[i]), 1);
+      mbar_init(smem_u32(&q_empty[i]), 16 + 4 + 2);  // every warp that reads the item
+      mbar_init(smem_u32(&i_full[i]), 1);
     }
     for (int i = 0; i < NK; ++i) {
       mbar_init(smem_u32(&k_full[i]), 1);
@@ -253,12 +312,12 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       mbar_init(smem_u32(&h_empty[i]), 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(smem_u32(&s_full[x]), 1);
+      for (int i = 0; i < TM::NS; ++i) mbar_init(smem_u32(&s_full[x * 2 + i]), 1);
       mbar_init(smem_u32(&p_full[x]), 256);
       mbar_init(smem_u32(&pv_done[x]), 1);
       mbar_init(smem_u32(&o_full[x]), 1);
     }
-    mbar_init(smem_u32(s_empty), 256);
+    for (int i = 0; i < TM::NS; ++i) mbar_init(smem_u32(&s_empty[i]), 256);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_q);
@@ -270,13 +329,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     tmem_relinquish<1>();
   }
   // ---- the sequences of this launch: one per thread, work items counted by a prefix sum
-  int items;
+  int entries;
   {
     PagedSeq s = {0, 0, 0};
-    int n = 0;
+    int n = 0, pairs = 0;
     const int i = threadIdx.x;
-    if (i < tp.seqs && paged_sequence(v, tp.seq0 + i, p.max_kv_len, &s) && s.T * p.group > p.rows_below)
-      n = (s.T + 2 * tp.tokens_per_tile - 1) / (2 * tp.tokens_per_tile) * splits_of(s.L, tp.chunk);
+    if (i < tp.seqs && paged_sequence(v, tp.seq0 + i, p.max_kv_len, &s) && s.T * p.group > p.rows_below) {
+      pairs = (s.T + 2 * tp.tokens_per_tile - 1) / (2 * tp.tokens_per_tile);
+      n = pairs * splits_of(s.L, tp.chunk);
+    }
     int sum = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -286,20 +347,18 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     if (lane == 31) warp_sum[warp] = sum;
     __syncthreads();
     int before = 0;
-    items = 0;
+    entries = 0;
     for (int k = 0; k < THREADS / 32; ++k) {
       if (k < warp) before += warp_sum[k];
-      items += warp_sum[k];
+      entries += warp_sum[k];
     }
-    items *= v.kv_heads;
-    if (i < MAX_SEQS) seq[i] = SeqInfo{s.q0, s.T, s.L, before + sum - n};
+    if (i < MAX_SEQS) seq[i] = SeqInfo{s.q0, s.T, s.L, before + sum - n, pairs};
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int G = p.group, TPT = tp.tokens_per_tile;
-  const int first = blockIdx.x, step = gridDim.x;
 
   if (warp >= 20) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
@@ -309,10 +368,18 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const int box = min(P, TILE), boxes = TILE / box;  // a 256-key page holds two tiles
       Ring rk, rv, rq;
       bool ok = true;
-      for (int idx = first; idx < items && ok; idx += step) {
-        const Item w = item_at(tp, seq, idx);
+      for (Walk walk(v.kv_heads, entries); ok; walk.next()) {
+        ok = wait_for(smem_u32(&q_empty[rq.stage]), rq.phase ^ 1, abort_flag, v.status, TI_ERR_PT_Q_EMPTY);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        Item w;
+        w.nt0 = -1;
+        if (walk.more()) w = item_at(tp, seq, walk);
+        if (lane == 0) {
+          *const_cast<Item*>(&item[rq.stage]) = w;
+          mbar_arrive(smem_u32(&i_full[rq.stage]));
+        }
+        if (w.nt0 < 0) break;
         const int n_tiles = max(w.nt0, w.nt1);
-        if (n_tiles == 0) continue;
         const int pages_used = (w.L + P - 1) >> v.page_shift;
         auto page_at = [&](int j) {  // page of this lane's rows of tile j; one past the pool (zeros) behind the last key
           const int i = (w.k0 + j * TILE + lane * box) >> v.page_shift;
@@ -320,9 +387,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           const int page = paged_page(v, w.b, i);
           return page < 0 ? 0 : page;
         };
-        int next = page_at(0);
-        ok = mbar_wait_status(smem_u32(&q_empty[rq.stage]), rq.phase ^ 1, abort_flag, v.status, TI_ERR_PT_Q_EMPTY);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        int next = n_tiles > 0 ? page_at(0) : 0;
         if (lane == 0) {
           const uint32_t bar = smem_u32(&q_full[rq.stage]);
           mbar_expect_tx(bar, ((w.nt0 > 0) + (w.nt1 > 0)) * G * TPT * 128);
@@ -336,7 +401,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           const int page = next;
           if (j + 1 < n_tiles) next = page_at(j + 1);
           const int row = (w.k0 + j * TILE + lane * box) & (P - 1);
-          ok = mbar_wait_status(smem_u32(&k_empty[rk.stage]), rk.phase ^ 1, abort_flag, v.status, TI_ERR_PT_K_EMPTY);
+          ok = wait_for(smem_u32(&k_empty[rk.stage]), rk.phase ^ 1, abort_flag, v.status, TI_ERR_PT_K_EMPTY);
           if (!__all_sync(0xffffffffu, ok)) break;
           if (lane == 0) mbar_expect_tx(smem_u32(&k_full[rk.stage]), TILE_BYTES);
           __syncwarp();
@@ -344,7 +409,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             tma_load_4d(smem_u32(smem + SM::K + rk.stage * TILE_BYTES + lane * box * 128), &tmap_k,
                         smem_u32(&k_full[rk.stage]), 0, row, w.h, page);
           rk.next(NK);
-          ok = mbar_wait_status(smem_u32(&v_empty[rv.stage]), rv.phase ^ 1, abort_flag, v.status, TI_ERR_PT_V_EMPTY);
+          ok = wait_for(smem_u32(&v_empty[rv.stage]), rv.phase ^ 1, abort_flag, v.status, TI_ERR_PT_V_EMPTY);
           if (!__all_sync(0xffffffffu, ok)) break;
           if (lane == 0) mbar_expect_tx(smem_u32(&v_full[rv.stage]), TILE_BYTES);
           __syncwarp();
@@ -361,34 +426,33 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const uint64_t desc = make_smem_desc_sw128(0);
       const uint32_t hi = static_cast<uint32_t>(desc >> 32), lo0 = static_cast<uint32_t>(desc);
       const uint32_t q_lo = lo0 + (smem_u32(smem + SM::Q) >> 4), k_lo = lo0 + (smem_u32(smem + SM::K) >> 4);
-      Ring rq, rk;
+      Ring rq, rk, rs;
       bool ok = true;
-      uint32_t s_parity = 1;  // the first wait passes at once
-      for (int idx = first; idx < items && ok; idx += step) {
-        const Item w = item_at(tp, seq, idx);
-        const int n_tiles = max(w.nt0, w.nt1);
-        if (n_tiles == 0) continue;
-        ok = mbar_wait_status(smem_u32(&q_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_Q);
+      while (ok) {
+        ok = wait_for(smem_u32(&i_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_ITEM);
+        const int nt0 = item[rq.stage].nt0, nt1 = item[rq.stage].nt1, n_tiles = max(nt0, nt1);
+        if (!ok || nt0 < 0) break;
+        mbar_arrive(smem_u32(&q_empty[rq.stage]));  // the item is read; its queries are kept by the softmax warps' arrivals
+        ok = wait_for(smem_u32(&q_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_Q);
         for (int j = 0; j < n_tiles && ok; ++j) {
-          ok = mbar_wait_status(smem_u32(&k_full[rk.stage]), rk.phase, abort_flag, v.status, TI_ERR_PT_K_FULL);
+          ok = wait_for(smem_u32(&k_full[rk.stage]), rk.phase, abort_flag, v.status, TI_ERR_PT_K_FULL);
           const uint32_t b_lo = k_lo + rk.stage * (TILE_BYTES >> 4);
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < 2; ++x) {
-            if (!ok || j >= (x ? w.nt1 : w.nt0)) continue;
-            ok = mbar_wait_status(smem_u32(s_empty), s_parity, abort_flag, v.status, TI_ERR_PT_S_EMPTY);
+            if (!ok || j >= (x ? nt1 : nt0)) continue;
+            ok = wait_for(smem_u32(&s_empty[rs.stage]), rs.phase ^ 1, abort_flag, v.status, TI_ERR_PT_S_EMPTY);
             if (!ok) continue;
-            s_parity ^= 1;
             tc_fence_after();
             const uint32_t a_lo = q_lo + (rq.stage * 2 + x) * (TILE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < (D + 31) / 32; ++k) umma_i8_lo(tmem + TMEM_S, a_lo + 2 * k, b_lo + 2 * k, hi, idesc, k != 0);
-            umma_commit(smem_u32(&s_full[x]));
+            for (int k = 0; k < (D + 31) / 32; ++k) umma_i8_lo(tmem + TM::S + rs.stage * TILE, a_lo + 2 * k, b_lo + 2 * k, hi, idesc, k != 0);
+            umma_commit(smem_u32(&s_full[x * 2 + rs.stage]));
+            rs.next(TM::NS);
           }
           if (!ok) break;
           umma_commit(smem_u32(&k_empty[rk.stage]));
           rk.next(NK);
         }
-        if (ok) umma_commit(smem_u32(&q_empty[rq.stage]));
         rq.next(NQ);
       }
     } else if (warp == 22 && lane == 0) {
@@ -397,26 +461,29 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const uint64_t desc = make_smem_desc_mn_sw128(0, TILE_BYTES);
       const uint32_t hi = static_cast<uint32_t>(desc >> 32);
       const uint32_t v_lo = static_cast<uint32_t>(desc) + (smem_u32(smem + SM::H) >> 4);
-      Ring rh;
+      Ring rq, rh;
       bool ok = true;
-      uint32_t p_phase[2] = {0, 0};
-      for (int idx = first; idx < items && ok; idx += step) {
-        const Item w = item_at(tp, seq, idx);
-        const int n_tiles = max(w.nt0, w.nt1);
+      uint32_t p_phase = 0;  // one bit per row tile
+      while (ok) {
+        ok = wait_for(smem_u32(&i_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_ITEM);
+        const int nt0 = item[rq.stage].nt0, nt1 = item[rq.stage].nt1, n_tiles = max(nt0, nt1);
+        if (!ok || nt0 < 0) break;
+        mbar_arrive(smem_u32(&q_empty[rq.stage]));
+        rq.next(NQ);
         for (int j = 0; j < n_tiles && ok; ++j) {
-          ok = mbar_wait_status(smem_u32(&h_full[rh.stage]), rh.phase, abort_flag, v.status, TI_ERR_PT_H_FULL);
+          ok = wait_for(smem_u32(&h_full[rh.stage]), rh.phase, abort_flag, v.status, TI_ERR_PT_H_FULL);
           const uint32_t b_lo = v_lo + rh.stage * (SM::HALF_BYTES >> 4);
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < 2; ++x) {
-            const int nt = x ? w.nt1 : w.nt0;
+            const int nt = x ? nt1 : nt0;
             if (!ok || j >= nt) continue;
-            ok = mbar_wait_status(smem_u32(&p_full[x]), p_phase[x], abort_flag, v.status, TI_ERR_PT_P_FULL);
+            ok = wait_for(smem_u32(&p_full[x]), (p_phase >> x) & 1, abort_flag, v.status, TI_ERR_PT_P_FULL);
             if (!ok) continue;
-            p_phase[x] ^= 1;
+            p_phase ^= 1u << x;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < TILE / 16; ++k)  // 16 keys of V are 2048 bytes
-              umma_f16_a_tmem(tmem + TMEM_O + x * TILE, tmem + TMEM_P + x * 64 + 8 * k, b_lo + k * (2048 >> 4), hi, idesc,
+              umma_f16_a_tmem(tmem + TM::O + x * TM::O_STRIDE, tmem + TM::P + x * 64 + 8 * k, b_lo + k * (2048 >> 4), hi, idesc,
                               j != 0 || k != 0);
             umma_commit(smem_u32(j + 1 < nt ? &pv_done[x] : &o_full[x]));
           }
@@ -434,14 +501,18 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     // 16-byte reads and writes fall into different banks.
     const int sub = lane >> 3, c = lane & 3;
     const int key8 = (lane >> 2) & 1 ? sub ^ 5 : sub;  // of a group of 8 keys
-    Ring rv, rh;
+    Ring rq, rv, rh;
     bool ok = true;
-    for (int idx = first; idx < items && ok; idx += step) {
-      const Item w = item_at(tp, seq, idx);
-      const int n_tiles = max(w.nt0, w.nt1);
+    while (ok) {
+      ok = wait_for(smem_u32(&i_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_ITEM);
+      const int nt0 = item[rq.stage].nt0, n_tiles = max(nt0, item[rq.stage].nt1);
+      if (!ok || nt0 < 0) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&q_empty[rq.stage]));
+      rq.next(NQ);
       for (int j = 0; j < n_tiles; ++j) {
-        ok = mbar_wait_status(smem_u32(&v_full[rv.stage]), rv.phase, abort_flag, v.status, TI_ERR_PT_V_FULL);
-        if (ok) ok = mbar_wait_status(smem_u32(&h_empty[rh.stage]), rh.phase ^ 1, abort_flag, v.status, TI_ERR_PT_H_EMPTY);
+        ok = wait_for(smem_u32(&v_full[rv.stage]), rv.phase, abort_flag, v.status, TI_ERR_PT_V_FULL);
+        if (ok) ok = wait_for(smem_u32(&h_empty[rh.stage]), rh.phase ^ 1, abort_flag, v.status, TI_ERR_PT_H_EMPTY);
         if (!ok) break;
         const uint8_t* src = smem + SM::V + rv.stage * TILE_BYTES;
         uint8_t* dst = smem + SM::H + rh.stage * SM::HALF_BYTES;
@@ -453,7 +524,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           *reinterpret_cast<uint4*>(row + ((o ^ (key & 7)) << 4)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
           *reinterpret_cast<uint4*>(row + (((o + 1) ^ (key & 7)) << 4)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
         };
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           const int key = (wv * 4 + i) * 8 + key8;
           convert(key, c);
@@ -472,44 +543,53 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     const int x = warp >> 3, half = (warp >> 2) & 1;   // row tile, 64 keys of a key tile
     const int r = (warp & 3) * 32 + lane;              // row of the tile = TMEM lane
-    const int r_token = r / G, r_head = r - r_token * G;
+    const int r_token = r / G;
     const int pair_bar = 1 + x * 4 + (warp & 3);       // barrier of the two warps that share 32 rows
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + TMEM_S + half * 64 + lane_off, tpp = tmem + TMEM_P + x * 64 + half * 32 + lane_off;
-    const uint32_t to = tmem + TMEM_O + x * TILE + half * (D / 2) + lane_off;  // this thread's columns of O
+    const uint32_t ts = tmem + TM::S + half * 64 + lane_off, tpp = tmem + TM::P + x * 64 + half * 32 + lane_off;
+    // this thread's columns of O, in sixteens: half of them (48 and 32 of 80)
+    const int col0 = half * (D == 80 ? 48 : D / 2), chunks = D == 80 ? 3 - half : D / 32;
+    const uint32_t to = tmem + TM::O + x * TM::O_STRIDE + col0 + lane_off;
     float* my_top = s_top + (x * 2 + half) * TILE + r;
     const float* other_top = s_top + (x * 2 + (half ^ 1)) * TILE + r;
     constexpr uint32_t kMagic = 0x4B400000u;           // bits of 1.5 * 2^23
     const float c = p.scale_log2;
     uint32_t s_phase = 0, pv_phase = 0, o_phase = 0;
-    // A wait that gives up (all later ones then return at once) does not leave the loops: the barriers of two warps
-    // have no limit, so both warps pass every one of them and only the results are not stored.
+    uint32_t s_base = 0;                               // score tiles of the items before this one
+    Ring rq;
+    // A wait that gives up (all later ones then return at once) does not leave an item: the barriers of two warps have
+    // no limit, so both warps pass every one of them and only the results are not stored.
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-      if (!mbar_wait_status(smem_u32(bar), parity, abort_flag, v.status, code)) ok = false;
-      __syncwarp();
+      if (!wait_for(smem_u32(bar), parity, abort_flag, v.status, code)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
     };
-    for (int idx = first; idx < items; idx += step) {
-      const Item w = item_at(tp, seq, idx);
-      const int tiles = x ? w.nt1 : w.nt0;
-      const int tile_t0 = w.t0 + x * TPT;
-      const int t = tile_t0 + r_token;
-      const int past = w.L - w.T;
-      const int lim = past + min(t, w.T - 1) - half * 64;  // last visible key, counted from this thread's columns
-      const int lim_min = past + tile_t0;
+    while (true) {
+      wait(&i_full[rq.stage], rq.phase, TI_ERR_PT_ITEM);
+      const int nt0 = item[rq.stage].nt0;
+      // both warps of a pair leave together (the sums of the item before have been read by now, too)
+      if (barrier_or(pair_bar, 64, !ok || nt0 < 0)) break;
+      const int nt1 = item[rq.stage].nt1;
+      const int tiles = x ? nt1 : nt0, others = x ? nt0 : nt1;
+      const int k0 = item[rq.stage].k0, T = item[rq.stage].T;
+      const int tile_t0 = item[rq.stage].t0 + x * TPT;
+      const int lim_min = item[rq.stage].L - T + tile_t0;                                            // last key of the first row
+      const int lim = lim_min + min(r_token, T - 1 - tile_t0) - half * 64;  // of this row, counted from this thread's columns
       float off = c * 12582912.f;
       float l = 0.f;
       for (int j = 0; j < tiles; ++j) {
-        wait(&s_full[x], s_phase, TI_ERR_PT_S_FULL);
-        s_phase ^= 1;
+        // the scores of a key tile are made for row tile 0, then 1, in buffers used in turn
+        const uint32_t buf = TM::NS == 1 ? 0 : (s_base + j + min(j + x, others)) % TM::NS;
+        wait(&s_full[x * 2 + buf], (s_phase >> buf) & 1, TI_ERR_PT_S_FULL);
+        s_phase ^= 1u << buf;
         tc_fence_after();
-        const int kt = w.k0 + j * TILE;
+        const int kt = k0 + j * TILE;
         uint32_t a[2][32];                             // scores, then their exponents
-        tmem_ld_32x32(ts, a[0]);
-        tmem_ld_32x32(ts + 32, a[1]);
+        tmem_ld_32x32(ts + buf * TILE, a[0]);
+        tmem_ld_32x32(ts + buf * TILE + 32, a[1]);
         tmem_ld_wait();
         tc_fence_before();
-        mbar_arrive(smem_u32(s_empty));
+        mbar_arrive(smem_u32(&s_empty[buf]));
         const float2 cc = make_float2(c, c), oo = make_float2(-off, -off);
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -526,14 +606,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             for (int i = 0; i < 32; ++i)
               if (kt + 32 * q + i > lim) a[q][i] = 0xFF800000u;
         }
-        float mx[4];
+        float mx[2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          mx[q] = __uint_as_float(a[q >> 1][(q & 1) * 16]);
+        for (int q = 0; q < 2; ++q) {
+          mx[q] = __uint_as_float(a[q][0]);
 #pragma unroll
-          for (int i = 1; i < 16; ++i) mx[q] = fmaxf(mx[q], __uint_as_float(a[q >> 1][(q & 1) * 16 + i]));
+          for (int i = 1; i < 31; i += 2) mx[q] = max3(mx[q], __uint_as_float(a[q][i]), __uint_as_float(a[q][i + 1]));
         }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        float top = max3(max3(mx[0], mx[1], __uint_as_float(a[0][31])), __uint_as_float(a[1][31]), -INFINITY);
         if (barrier_or(pair_bar, 64, j == 0 || top > 15.f)) {
           *my_top = top;
           asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
@@ -556,7 +636,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             wait(&pv_done[x], pv_phase, TI_ERR_PT_PV);
             tc_fence_after();
 #pragma unroll 1
-            for (int q = 0; q < D / 16; ++q) {
+            for (int q = 0; q < 2 * chunks; ++q) {
               uint32_t o[8];
               tmem_ld_32x8(to + 8 * q, o);
               tmem_ld_wait();
@@ -593,40 +673,75 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         o_phase ^= 1;
         tc_fence_after();
       }
-      if (w.split >= w.n_splits) continue;             // beyond the keys of this pair of row tiles
+      s_base += tiles + others;
       s_sum[(x * 2 + half) * TILE + r] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l = s_sum[x * 2 * TILE + r] + s_sum[(x * 2 + 1) * TILE + r];
-      const bool valid = ok && r < G * TPT && t < w.T;
-      const long long at = static_cast<long long>(w.q0 + t) * p.q_heads + w.h * G + r_head;
-      const bool whole = w.n_splits == 1;
+      // The item is read again and `row` is opaque, so that nothing of this is carried through the loop above.
+      int row = r;
+      asm volatile("" : "+r"(row));
+      const int split = item[rq.stage].split, n_splits = item[rq.stage].n_splits;
+      const int token = row / G, t = item[rq.stage].t0 + x * TPT + token;
+      // beyond the keys of this pair of row tiles there is nothing to write
+      const bool valid = ok && row < G * TPT && t < item[rq.stage].T && split < n_splits;
+      const long long at = static_cast<long long>(item[rq.stage].q0 + t) * p.q_heads + item[rq.stage].h * G + (row - token * G);
+      const bool whole = n_splits == 1;
       const float scale = l > 0.f ? p.alpha_pv / l : 0.f;
-      float* po = p.part_o + (at * p.max_splits + w.split) * D + half * (D / 2);
-      if (valid && !whole && half == 0) p.part_ml[at * p.max_splits + w.split] = make_float2(l > 0.f ? off : -1e30f, l);
+      const long long part = at * p.max_splits + split;
+      if (valid && !whole && half == 0) p.part_ml[part] = make_float2(l > 0.f ? off : -1e30f, l);
+      // Context rows.  A thread holds a row; stored from there, a warp would touch 32 rows with every instruction
+      // (measured: 4700 clocks for the two row tiles).  So 64 bytes of each row at a time pass through shared memory -
+      // the item's query tile, which nobody reads any more - and every group of four lanes stores one row's.
+      uint8_t* out = whole ? static_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
+      const int width = !whole ? 4 : p.out_kind == 3 ? 1 : 2;  // bytes of an element
+      const long long row_bytes = (whole ? at : part) * D * width + col0 * width;
+      const int per_round = 4 / width;                         // sixteens of columns in 64 bytes
+      const bool staged = tiles + others > 0;
+      uint8_t* stage = smem + SM::Q + (rq.stage * 2 + x) * TILE_BYTES + (half * 4 + (warp & 3)) * 2048;
 #pragma unroll 1
-      for (int q = 0; q < D / 16; ++q) {
-        uint32_t o[8];
-        if (tiles > 0) {
-          tmem_ld_32x8(to + 8 * q, o);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = 0;
-        }
-        if (valid) {
-          if (whole) {
-            paged_store8(p, at * D + half * (D / 2) + 8 * q, o, scale);
+      for (int q0 = 0; q0 < chunks; q0 += per_round) {
+        const int n = min(per_round, chunks - q0);
+#pragma unroll 1
+        for (int q = 0; q < n; ++q) {
+          uint32_t o[16];
+          if (tiles > 0) {
+            tmem_ld_32x16(to + 16 * (q0 + q), o);
+            tmem_ld_wait();
           } else {
-            *reinterpret_cast<uint4*>(po + 8 * q) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(po + 8 * q + 4) = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = 0;
+          }
+          uint4 piece[4];
+          paged_convert16(width, p.out_kind, o, scale, piece);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k >= width) continue;
+            const int c16 = q * width + k;                     // 16-byte piece of the round
+            if (staged)
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((c16 ^ ((lane >> 1) & 3)) << 4)) = piece[k];
+            else if (valid)
+              *reinterpret_cast<uint4*>(out + row_bytes + (q0 * width + c16) * 16) = piece[k];
+          }
+        }
+        __syncwarp();
+        if (staged) {
+          const int c16 = lane & 3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = i * 8 + (lane >> 2);
+            const long long base = __shfl_sync(0xffffffffu, row_bytes, rr);
+            const bool there = __shfl_sync(0xffffffffu, static_cast<int>(valid), rr) != 0;
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c16 ^ ((rr >> 1) & 3)) << 4));
+            if (there && c16 < n * width) *reinterpret_cast<uint4*>(out + base + (q0 * width + c16) * 16) = y;
           }
         }
         __syncwarp();
       }
-      // the next item's sums are written after its barriers, and its products overwrite O only after this thread's
-      // next arrival on p_full
-      tc_fence_before();
-      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&q_empty[rq.stage]));
+      rq.next(NQ);
+      tc_fence_before();  // the next item's products overwrite O only after this thread's next arrival on p_full
     }
   }
 
