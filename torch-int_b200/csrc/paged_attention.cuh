@@ -49,63 +49,33 @@ __device__ __forceinline__ PagedSplits paged_splits(int keys, int chunk) {
   return s;
 }
 
-// Four neighbouring context values times `scale`, rounded once to the output type.
+// Context values rounded once to the output type: two to fp16 or bf16, four to int8 (rne, saturated).
+__device__ __forceinline__ uint32_t paged_pack2(int out_kind, float a, float b) {
+  uint32_t r;
+  if (out_kind == 2)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t paged_pack4_s8(float a, float b, float c, float d) {
+  uint32_t lo, w;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(lo));
+  return w;
+}
+
+// Four neighbouring context values times `scale`.
 __device__ __forceinline__ void paged_store4(const PagedAttnParams& p, long long at, float4 x, float scale) {
   x.x *= scale;
   x.y *= scale;
   x.z *= scale;
   x.w *= scale;
-  if (p.out_kind == 3) {
-    uint32_t lo, w;
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(x.w)), "r"(__float2int_rn(x.z)));
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(lo));
-    *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.out) + at) = w;
-  } else if (p.out_kind == 2) {
-    const __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
-  } else {
-    const __half2 u = __floats2half2_rn(x.x, x.y), w = __floats2half2_rn(x.z, x.w);
-    *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
-  }
-}
-
-// Sixteen neighbouring context values (fp32 bits) as `width` 16-byte pieces: 4 as they are (a partial result), 2 and
-// 1 times `scale` and rounded once to fp16 / bf16 and int8.
-__device__ __forceinline__ void paged_convert16(int width, int out_kind, const uint32_t (&o)[16], float scale, uint4 (&piece)[4]) {
-  if (width == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) piece[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-    return;
-  }
-  float x[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(o[i]) * scale;
-  uint32_t w[8];
-  if (width == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t lo;
-      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(x[4 * i + 3])), "r"(__float2int_rn(x[4 * i + 2])));
-      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;"
-          : "=r"(w[i]) : "r"(__float2int_rn(x[4 * i + 1])), "r"(__float2int_rn(x[4 * i])), "r"(lo));
-    }
-  } else if (out_kind == 2) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half2 u = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&u);
-    }
-  }
-  piece[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  if (width == 2) piece[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  if (p.out_kind == 3)
+    *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.out) + at) = paged_pack4_s8(x.x, x.y, x.z, x.w);
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+        make_uint2(paged_pack2(p.out_kind, x.x, x.y), paged_pack2(p.out_kind, x.z, x.w));
 }
 
 }  // namespace ti

@@ -547,8 +547,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int pair_bar = 1 + x * 4 + (warp & 3);       // barrier of the two warps that share 32 rows
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + TM::S + half * 64 + lane_off, tpp = tmem + TM::P + x * 64 + half * 32 + lane_off;
-    // this thread's columns of O, in sixteens: half of them (48 and 32 of 80)
-    const int col0 = half * (D == 80 ? 48 : D / 2), chunks = D == 80 ? 3 - half : D / 32;
+    // this thread's columns of O: half of them (48 and 32 of 80)
+    const int col0 = half * (D == 80 ? 48 : D / 2), cols = D == 80 ? 48 - 16 * half : D / 2;
     const uint32_t to = tmem + TM::O + x * TM::O_STRIDE + col0 + lane_off;
     float* my_top = s_top + (x * 2 + half) * TILE + r;
     const float* other_top = s_top + (x * 2 + (half ^ 1)) * TILE + r;
@@ -636,13 +636,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             wait(&pv_done[x], pv_phase, TI_ERR_PT_PV);
             tc_fence_after();
 #pragma unroll 1
-            for (int q = 0; q < 2 * chunks; ++q) {
+            for (int col = 0; col < cols; col += 8) {
               uint32_t o[8];
-              tmem_ld_32x8(to + 8 * q, o);
+              tmem_ld_32x8(to + col, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st_32x8(to + 8 * q, o);
+              tmem_st_32x8(to + col, o);
             }
           }
         }
@@ -681,61 +681,58 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       int row = r;
       asm volatile("" : "+r"(row));
       const int split = item[rq.stage].split, n_splits = item[rq.stage].n_splits;
-      const int token = row / G, t = item[rq.stage].t0 + x * TPT + token;
+      const int t = item[rq.stage].t0 + x * TPT + r_token;
       // beyond the keys of this pair of row tiles there is nothing to write
       const bool valid = ok && row < G * TPT && t < item[rq.stage].T && split < n_splits;
-      const long long at = static_cast<long long>(item[rq.stage].q0 + t) * p.q_heads + item[rq.stage].h * G + (row - token * G);
       const bool whole = n_splits == 1;
-      const float scale = l > 0.f ? p.alpha_pv / l : 0.f;
-      const long long part = at * p.max_splits + split;
-      if (valid && !whole && half == 0) p.part_ml[part] = make_float2(l > 0.f ? off : -1e30f, l);
-      // Context rows.  A thread holds a row; stored from there, a warp would touch 32 rows with every instruction
-      // (measured: 4700 clocks for the two row tiles).  So 64 bytes of each row at a time pass through shared memory -
-      // the item's query tile, which nobody reads any more - and every group of four lanes stores one row's.
-      uint8_t* out = whole ? static_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
+      long long at = static_cast<long long>(item[rq.stage].q0 + t) * p.q_heads + item[rq.stage].h * G + (row - r_token * G);
+      if (!whole) at = at * p.max_splits + split;
+      const float scale = !whole ? 1.f : l > 0.f ? p.alpha_pv / l : 0.f;
+      if (valid && !whole && half == 0) p.part_ml[at] = make_float2(l > 0.f ? off : -1e30f, l);
+      // Context rows.  A thread holds a row; stored from there, a warp would touch 32 rows with every instruction.  So
+      // 64 bytes of each row at a time pass through shared memory - the item's query tile, which nobody reads any more -
+      // and every group of four lanes stores one row's.  Loops of few instructions: this code is cold each time it is
+      // reached, and fetching it unrolled took longer (4200 clocks) than the stores.
       const int width = !whole ? 4 : p.out_kind == 3 ? 1 : 2;  // bytes of an element
-      const long long row_bytes = (whole ? at : part) * D * width + col0 * width;
-      const int per_round = 4 / width;                         // sixteens of columns in 64 bytes
-      const bool staged = tiles + others > 0;
+      uint8_t* out = whole ? static_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
+      const long long row_bytes = (at * D + col0) * width;
       uint8_t* stage = smem + SM::Q + (rq.stage * 2 + x) * TILE_BYTES + (half * 4 + (warp & 3)) * 2048;
 #pragma unroll 1
-      for (int q0 = 0; q0 < chunks; q0 += per_round) {
-        const int n = min(per_round, chunks - q0);
-#pragma unroll 1
-        for (int q = 0; q < n; ++q) {
-          uint32_t o[16];
-          if (tiles > 0) {
-            tmem_ld_32x16(to + 16 * (q0 + q), o);
-            tmem_ld_wait();
-          } else {
+      for (int col = 0; col < cols; col += 8) {
+        uint32_t o[8];
+        tmem_ld_32x8(to + col, o);
+        tmem_ld_wait();
+        float y[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0;
-          }
-          uint4 piece[4];
-          paged_convert16(width, p.out_kind, o, scale, piece);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k >= width) continue;
-            const int c16 = q * width + k;                     // 16-byte piece of the round
-            if (staged)
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((c16 ^ ((lane >> 1) & 3)) << 4)) = piece[k];
-            else if (valid)
-              *reinterpret_cast<uint4*>(out + row_bytes + (q0 * width + c16) * 16) = piece[k];
-          }
+        for (int i = 0; i < 8; ++i) y[i] = tiles > 0 ? __uint_as_float(o[i]) * scale : 0.f;
+        const int byte = (col * width) & 63;
+        const int piece = byte >> 4, swz = (lane >> 1) & 3;
+        uint8_t* dst = stage + lane * 64;
+        if (width == 4) {
+          *reinterpret_cast<float4*>(dst + ((piece ^ swz) << 4)) = make_float4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<float4*>(dst + (((piece + 1) ^ swz) << 4)) = make_float4(y[4], y[5], y[6], y[7]);
+        } else if (width == 2) {
+          *reinterpret_cast<uint4*>(dst + ((piece ^ swz) << 4)) =
+              make_uint4(paged_pack2(p.out_kind, y[0], y[1]), paged_pack2(p.out_kind, y[2], y[3]),
+                         paged_pack2(p.out_kind, y[4], y[5]), paged_pack2(p.out_kind, y[6], y[7]));
+        } else {
+          *reinterpret_cast<uint2*>(dst + ((piece ^ swz) << 4) + (byte & 8)) =
+              make_uint2(paged_pack4_s8(y[0], y[1], y[2], y[3]), paged_pack4_s8(y[4], y[5], y[6], y[7]));
         }
-        __syncwarp();
-        if (staged) {
-          const int c16 = lane & 3;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = i * 8 + (lane >> 2);
+        if (byte + 8 * width == 64 || col + 8 == cols) {
+          __syncwarp();
+          const int done = col * width - byte, c16 = (lane & 3) * 16;
+#pragma unroll 1
+          for (int i = 0; i < 32; i += 8) {
+            const int rr = i + (lane >> 2);
             const long long base = __shfl_sync(0xffffffffu, row_bytes, rr);
             const bool there = __shfl_sync(0xffffffffu, static_cast<int>(valid), rr) != 0;
-            const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c16 ^ ((rr >> 1) & 3)) << 4));
-            if (there && c16 < n * width) *reinterpret_cast<uint4*>(out + base + (q0 * width + c16) * 16) = y;
+            if (there && c16 < byte + 8 * width)
+              *reinterpret_cast<uint4*>(out + base + done + c16) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 64 + (c16 ^ (((rr >> 1) & 3) << 4)));
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
