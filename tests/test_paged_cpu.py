@@ -15,6 +15,35 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB = os.path.join(ROOT, "torch-int_b200", "torch_int", "lib", "libtorch_int_b200.so")
 
 
+I_, F_, P_ = ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+
+
+class PagedBatch(ctypes.Structure):
+    # struct ti_paged_batch
+    _fields_ = [
+        ("k_pages", P_), ("v_pages", P_), ("block_table", P_), ("query_starts", P_), ("kv_lens", P_),
+        ("num_pages", I_), ("kv_heads", I_), ("page_size", I_), ("head_dim", I_),
+        ("table_stride", I_), ("table_width", I_), ("batch", I_), ("tokens", I_), ("max_query_len", I_),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    # struct ti_paged_append_args
+    _fields_ = [
+        ("q", P_), ("k", P_), ("v", P_), ("ld_q", I_), ("ld_k", I_), ("ld_v", I_), ("q_heads", I_),
+        ("rotary", P_), ("rotary_rows", I_), ("rotary_dim", I_), ("q_out", P_),
+        ("q_alpha", F_), ("k_alpha", F_), ("v_alpha", F_), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    # struct ti_paged_attention_args
+    _fields_ = [
+        ("q", P_), ("ld_q", I_), ("q_heads", I_), ("max_kv_len", I_), ("out", P_), ("workspace", P_),
+        ("workspace_bytes", I_), ("alpha_qk", F_), ("alpha_pv", F_), ("out_kind", ctypes.c_int32),
+    ]
+
+
 @pytest.fixture(scope="module")
 def lib():
     lib = ctypes.CDLL(LIB)
@@ -33,7 +62,7 @@ def batch_of(base, **kw):
     b = dict(k_pages=base, v_pages=base, block_table=base, query_starts=base, kv_lens=base, num_pages=4, kv_heads=2,
              page_size=16, head_dim=64, table_stride=4, table_width=4, batch=2, tokens=3, max_query_len=2)
     b.update(kw)
-    return C._PagedBatch(**b)
+    return PagedBatch(**b)
 
 
 @pytest.mark.parametrize("change,words", [
@@ -46,8 +75,8 @@ def batch_of(base, **kw):
 def test_bad_batches_are_refused(lib, base, change, words):
     """Before any CUDA call, by both entry points."""
     b = batch_of(base, **{k: (base + v if k in ("v_pages", "query_starts") else v) for k, v in change.items()})
-    att = C._PagedAttentionArgs(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1)
-    app = C._PagedAppendArgs(k=base, v=base, ld_k=128, ld_v=128, dtype=3)
+    att = PagedAttentionArgs(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1)
+    app = PagedAppendArgs(k=base, v=base, ld_k=128, ld_v=128, dtype=3)
     assert lib.ti_paged_attention(ctypes.byref(b), ctypes.byref(att), None) == -1 and words in lib.ti_last_error()
     assert lib.ti_paged_append(ctypes.byref(b), ctypes.byref(app), None) == -1 and words in lib.ti_last_error()
 
@@ -61,7 +90,7 @@ def test_bad_batches_are_refused(lib, base, change, words):
 def test_bad_attention_arguments_are_refused(lib, base, change, words):
     a = dict(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1, alpha_qk=1.0, alpha_pv=1.0)
     a.update(change)
-    args = C._PagedAttentionArgs(**a)
+    args = PagedAttentionArgs(**a)
     assert lib.ti_paged_attention(ctypes.byref(batch_of(base)), ctypes.byref(args), None) == -1
     assert words in lib.ti_last_error()
 
@@ -74,20 +103,30 @@ def test_bad_attention_arguments_are_refused(lib, base, change, words):
 def test_bad_append_arguments_are_refused(lib, base, change, words):
     a = dict(k=base, v=base, ld_k=128, ld_v=128, dtype=3, k_alpha=1.0, v_alpha=1.0)
     a.update({k: (base if v == "base" else v) for k, v in change.items()})
-    args = C._PagedAppendArgs(**a)
+    args = PagedAppendArgs(**a)
     assert lib.ti_paged_append(ctypes.byref(batch_of(base)), ctypes.byref(args), None) == -1
     assert words in lib.ti_last_error()
 
 
 def test_null_descriptors_and_empty_calls(lib, base):
-    att = C._PagedAttentionArgs(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1)
-    app = C._PagedAppendArgs(k=base, v=base, ld_k=128, ld_v=128, dtype=3)
+    att = PagedAttentionArgs(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1)
+    app = PagedAppendArgs(k=base, v=base, ld_k=128, ld_v=128, dtype=3)
     assert lib.ti_paged_attention(None, ctypes.byref(att), None) == -1
     assert lib.ti_paged_append(ctypes.byref(batch_of(base)), None, None) == -1
     for kw in (dict(tokens=0), dict(batch=0), dict(max_query_len=0)):  # accepted, nothing launched
         b = batch_of(base, **kw)
         assert lib.ti_paged_attention(ctypes.byref(b), ctypes.byref(att), None) == 0
         assert lib.ti_paged_append(ctypes.byref(b), ctypes.byref(app), None) == 0
+
+
+def test_packed_descriptors_match_the_structs():
+    """The bytes that the Python entry points pass are those of the C structs, field by field."""
+    n = range(1, 15)
+    assert C._pack_paged_batch(*n) == bytes(PagedBatch(*n))
+    a = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 0.5, 0.25, 0.125, 2, 1)
+    assert C._pack_paged_append(*a) == bytes(PagedAppendArgs(*a))
+    a = (1, 2, 3, 4, 5, 6, 7, 0.5, 0.25, 3)
+    assert C._pack_paged_attention(*a) == bytes(PagedAttentionArgs(*a))
 
 
 def test_workspace_query():

@@ -55,13 +55,7 @@ constexpr int THREADS = 768;
 constexpr int TMEM_COLS = 512;
 constexpr int REGS_SOFTMAX = 96, REGS_CONVERT = 48, REGS_OTHER = 48;  // per thread, of 768 x 80 at launch
 
-// Columns of TMEM: scores (64-wide heads leave room for a second buffer), P of both row tiles, O of both.
-template <int D>
-struct Tmem {
-  static constexpr int NS = D == 64 ? 2 : 1;
-  static constexpr uint32_t S = 0, P = NS * TILE, O = P + 2 * 64, O_STRIDE = D == 64 ? 64 : 128;
-  static_assert(O + 2 * O_STRIDE <= TMEM_COLS, "512 columns");
-};
+constexpr uint32_t TMEM_S = 0, TMEM_P = 128, TMEM_O = 256;  // P + 64, O + 128 for row tile 1
 
 template <int D>
 struct Smem {
@@ -265,7 +259,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const PagedAttnParams& p = tp.a;
   const PagedView& v = p.view;
   using SM = Smem<D>;
-  using TM = Tmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   SeqInfo* seq = reinterpret_cast<SeqInfo*>(smem + SM::SEQ);
@@ -281,8 +274,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint64_t* h_full = v_empty + NV;
   uint64_t* h_empty = h_full + NH;
   uint64_t* s_full = h_empty + NH;
-  uint64_t* s_empty = s_full + 4;  // s_full: [row tile][buffer], s_empty: [buffer]
-  uint64_t* p_full = s_empty + 2;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_empty + 1;
   uint64_t* pv_done = p_full + 2;
   uint64_t* o_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
@@ -312,12 +305,12 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       mbar_init(smem_u32(&h_empty[i]), 1);
     }
     for (int x = 0; x < 2; ++x) {
-      for (int i = 0; i < TM::NS; ++i) mbar_init(smem_u32(&s_full[x * 2 + i]), 1);
+      mbar_init(smem_u32(&s_full[x]), 1);
       mbar_init(smem_u32(&p_full[x]), 256);
       mbar_init(smem_u32(&pv_done[x]), 1);
       mbar_init(smem_u32(&o_full[x]), 1);
     }
-    for (int i = 0; i < TM::NS; ++i) mbar_init(smem_u32(&s_empty[i]), 256);
+    mbar_init(smem_u32(s_empty), 256);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_q);
@@ -426,7 +419,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const uint64_t desc = make_smem_desc_sw128(0);
       const uint32_t hi = static_cast<uint32_t>(desc >> 32), lo0 = static_cast<uint32_t>(desc);
       const uint32_t q_lo = lo0 + (smem_u32(smem + SM::Q) >> 4), k_lo = lo0 + (smem_u32(smem + SM::K) >> 4);
-      Ring rq, rk, rs;
+      Ring rq, rk;
+      uint32_t s_parity = 1;  // the first wait passes at once
       bool ok = true;
       while (ok) {
         ok = wait_for(smem_u32(&i_full[rq.stage]), rq.phase, abort_flag, v.status, TI_ERR_PT_ITEM);
@@ -440,14 +434,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll 1
           for (int x = 0; x < 2; ++x) {
             if (!ok || j >= (x ? nt1 : nt0)) continue;
-            ok = wait_for(smem_u32(&s_empty[rs.stage]), rs.phase ^ 1, abort_flag, v.status, TI_ERR_PT_S_EMPTY);
+            ok = wait_for(smem_u32(s_empty), s_parity, abort_flag, v.status, TI_ERR_PT_S_EMPTY);
             if (!ok) continue;
+            s_parity ^= 1;
             tc_fence_after();
             const uint32_t a_lo = q_lo + (rq.stage * 2 + x) * (TILE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < (D + 31) / 32; ++k) umma_i8_lo(tmem + TM::S + rs.stage * TILE, a_lo + 2 * k, b_lo + 2 * k, hi, idesc, k != 0);
-            umma_commit(smem_u32(&s_full[x * 2 + rs.stage]));
-            rs.next(TM::NS);
+            for (int k = 0; k < (D + 31) / 32; ++k) umma_i8_lo(tmem + TMEM_S, a_lo + 2 * k, b_lo + 2 * k, hi, idesc, k != 0);
+            umma_commit(smem_u32(&s_full[x]));
           }
           if (!ok) break;
           umma_commit(smem_u32(&k_empty[rk.stage]));
@@ -483,7 +477,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < TILE / 16; ++k)  // 16 keys of V are 2048 bytes
-              umma_f16_a_tmem(tmem + TM::O + x * TM::O_STRIDE, tmem + TM::P + x * 64 + 8 * k, b_lo + k * (2048 >> 4), hi, idesc,
+              umma_f16_a_tmem(tmem + TMEM_O + x * TILE, tmem + TMEM_P + x * 64 + 8 * k, b_lo + k * (2048 >> 4), hi, idesc,
                               j != 0 || k != 0);
             umma_commit(smem_u32(j + 1 < nt ? &pv_done[x] : &o_full[x]));
           }
@@ -524,7 +518,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           *reinterpret_cast<uint4*>(row + ((o ^ (key & 7)) << 4)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
           *reinterpret_cast<uint4*>(row + (((o + 1) ^ (key & 7)) << 4)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
         };
-#pragma unroll 1
+#pragma unroll 2
         for (int i = 0; i < 4; ++i) {
           const int key = (wv * 4 + i) * 8 + key8;
           convert(key, c);
@@ -546,16 +540,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int r_token = r / G;
     const int pair_bar = 1 + x * 4 + (warp & 3);       // barrier of the two warps that share 32 rows
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + TM::S + half * 64 + lane_off, tpp = tmem + TM::P + x * 64 + half * 32 + lane_off;
+    const uint32_t ts = tmem + TMEM_S + half * 64 + lane_off, tpp = tmem + TMEM_P + x * 64 + half * 32 + lane_off;
     // this thread's columns of O: half of them (48 and 32 of 80)
     const int col0 = half * (D == 80 ? 48 : D / 2), cols = D == 80 ? 48 - 16 * half : D / 2;
-    const uint32_t to = tmem + TM::O + x * TM::O_STRIDE + col0 + lane_off;
+    const uint32_t to = tmem + TMEM_O + x * TILE + col0 + lane_off;
     float* my_top = s_top + (x * 2 + half) * TILE + r;
     const float* other_top = s_top + (x * 2 + (half ^ 1)) * TILE + r;
     constexpr uint32_t kMagic = 0x4B400000u;           // bits of 1.5 * 2^23
     const float c = p.scale_log2;
     uint32_t s_phase = 0, pv_phase = 0, o_phase = 0;
-    uint32_t s_base = 0;                               // score tiles of the items before this one
     Ring rq;
     // A wait that gives up (all later ones then return at once) does not leave an item: the barriers of two warps have
     // no limit, so both warps pass every one of them and only the results are not stored.
@@ -570,7 +563,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       // both warps of a pair leave together (the sums of the item before have been read by now, too)
       if (barrier_or(pair_bar, 64, !ok || nt0 < 0)) break;
       const int nt1 = item[rq.stage].nt1;
-      const int tiles = x ? nt1 : nt0, others = x ? nt0 : nt1;
+      const int tiles = x ? nt1 : nt0;
       const int k0 = item[rq.stage].k0, T = item[rq.stage].T;
       const int tile_t0 = item[rq.stage].t0 + x * TPT;
       const int lim_min = item[rq.stage].L - T + tile_t0;                                            // last key of the first row
@@ -578,18 +571,16 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       float off = c * 12582912.f;
       float l = 0.f;
       for (int j = 0; j < tiles; ++j) {
-        // the scores of a key tile are made for row tile 0, then 1, in buffers used in turn
-        const uint32_t buf = TM::NS == 1 ? 0 : (s_base + j + min(j + x, others)) % TM::NS;
-        wait(&s_full[x * 2 + buf], (s_phase >> buf) & 1, TI_ERR_PT_S_FULL);
-        s_phase ^= 1u << buf;
+        wait(&s_full[x], s_phase, TI_ERR_PT_S_FULL);
+        s_phase ^= 1;
         tc_fence_after();
         const int kt = k0 + j * TILE;
         uint32_t a[2][32];                             // scores, then their exponents
-        tmem_ld_32x32(ts + buf * TILE, a[0]);
-        tmem_ld_32x32(ts + buf * TILE + 32, a[1]);
+        tmem_ld_32x32(ts, a[0]);
+        tmem_ld_32x32(ts + 32, a[1]);
         tmem_ld_wait();
         tc_fence_before();
-        mbar_arrive(smem_u32(&s_empty[buf]));
+        mbar_arrive(smem_u32(s_empty));
         const float2 cc = make_float2(c, c), oo = make_float2(-off, -off);
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -673,7 +664,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         o_phase ^= 1;
         tc_fence_after();
       }
-      s_base += tiles + others;
       s_sum[(x * 2 + half) * TILE + r] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l = s_sum[x * 2 * TILE + r] + s_sum[(x * 2 + 1) * TILE + r];

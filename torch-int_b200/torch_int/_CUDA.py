@@ -21,6 +21,7 @@ Extra callables (not in the reference) are listed at the end of ``__all__``.
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -69,32 +70,6 @@ class _GemmDesc(ctypes.Structure):
     ]
 
 
-class _PagedBatch(ctypes.Structure):
-    # struct ti_paged_batch
-    _fields_ = [
-        ("k_pages", _ptr), ("v_pages", _ptr), ("block_table", _ptr), ("query_starts", _ptr), ("kv_lens", _ptr),
-        ("num_pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64),
-        ("table_stride", _i64), ("table_width", _i64), ("batch", _i64), ("tokens", _i64), ("max_query_len", _i64),
-    ]
-
-
-class _PagedAppendArgs(ctypes.Structure):
-    # struct ti_paged_append_args
-    _fields_ = [
-        ("q", _ptr), ("k", _ptr), ("v", _ptr), ("ld_q", _i64), ("ld_k", _i64), ("ld_v", _i64), ("q_heads", _i64),
-        ("rotary", _ptr), ("rotary_rows", _i64), ("rotary_dim", _i64), ("q_out", _ptr),
-        ("q_alpha", _f32), ("k_alpha", _f32), ("v_alpha", _f32), ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32),
-    ]
-
-
-class _PagedAttentionArgs(ctypes.Structure):
-    # struct ti_paged_attention_args
-    _fields_ = [
-        ("q", _ptr), ("ld_q", _i64), ("q_heads", _i64), ("max_kv_len", _i64), ("out", _ptr), ("workspace", _ptr),
-        ("workspace_bytes", _i64), ("alpha_qk", _f32), ("alpha_pv", _f32), ("out_kind", ctypes.c_int32),
-    ]
-
-
 def _sig(name, argtypes, restype=ctypes.c_int):
     fn = getattr(_lib, name)
     fn.argtypes = argtypes
@@ -134,8 +109,12 @@ _c_attention_prefill = _sig("ti_attention_prefill_s8",
                             [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64,
                              _i64, _i64, _i64, _i64, _i64, _f32, _f32, _ptr])
 _c_transpose_values = _sig("ti_transpose_values", [_ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr])
-_c_paged_append = _sig("ti_paged_append", [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_PagedAppendArgs), _ptr])
-_c_paged_attention = _sig("ti_paged_attention", [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_PagedAttentionArgs), _ptr])
+# The paged operators serve single tokens, where the host side counts: their structs are packed as bytes.
+_c_paged_append = _sig("ti_paged_append", [ctypes.c_char_p, ctypes.c_char_p, _ptr])
+_c_paged_attention = _sig("ti_paged_attention", [ctypes.c_char_p, ctypes.c_char_p, _ptr])
+_pack_paged_batch = struct.Struct("=5Q9q").pack             # struct ti_paged_batch
+_pack_paged_append = struct.Struct("=3Q4qQ2qQ3f2i4x").pack  # struct ti_paged_append_args
+_pack_paged_attention = struct.Struct("=Q3q2Qq2fi4x").pack  # struct ti_paged_attention_args
 _c_paged_workspace = _sig("ti_paged_attention_workspace_bytes", [_i64] * 7, _i64)
 _c_last_error = _sig("ti_last_error", [], ctypes.c_char_p)
 _c_device_status = _sig("ti_device_status", [ctypes.POINTER(ctypes.c_int), _i32])
@@ -192,8 +171,14 @@ def _check(rc):
     launch_count += 1
 
 
+# the handle alone, without the Stream object that torch.cuda.current_stream() builds (4 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _stream_ptr(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 class _on_device:
@@ -206,7 +191,7 @@ class _on_device:
         self.prev = None
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = _current_device()
         if cur != self.idx:
             self.prev = cur
             torch.cuda.set_device(self.idx)
@@ -642,48 +627,68 @@ def transpose_values(v, vt, col0=0):
     return vt
 
 
+_PAGED_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+
+
 def _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, tokens, max_query_len):
-    """Checks the cache and the index tensors of a ragged batch; returns (descriptor, device, kv_heads, head_dim)."""
-    if not (isinstance(k_pages, torch.Tensor) and isinstance(v_pages, torch.Tensor) and k_pages.is_cuda
-            and k_pages.dtype == torch.int8 and v_pages.dtype == torch.int8 and k_pages.dim() == 4
-            and k_pages.shape == v_pages.shape and k_pages.device == v_pages.device
+    """Checks the cache and the index tensors of a ragged batch; returns the packed ti_paged_batch, the device index
+    and the sizes (sequences, heads, page_size, head_dim, block table width, bound of the new tokens)."""
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"),
+                    (query_starts, "query_starts"), (kv_lens, "kv_lens")):
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{name} must be a torch.Tensor")
+    shape = k_pages.shape
+    dev = k_pages.get_device()
+    if not (dev >= 0 and len(shape) == 4 and k_pages.dtype is torch.int8 and v_pages.dtype is torch.int8
+            and v_pages.shape == shape and v_pages.get_device() == dev
             and k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise RuntimeError("k_pages and v_pages must be contiguous CUDA int8 tensors of the same shape "
                            "[pages, kv_heads, page_size, head_dim]")
-    pages, hkv, page_size, d = k_pages.shape
-    dev = k_pages.device
-    for t, name in ((block_table, "block_table"), (query_starts, "query_starts"), (kv_lens, "kv_lens")):
-        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == dev):
-            raise RuntimeError(f"{name} must be an int32 tensor on {dev}")
-    if block_table.dim() != 2 or query_starts.dim() != 1 or kv_lens.dim() != 1 \
-            or query_starts.shape[0] != kv_lens.shape[0] + 1 or block_table.shape[0] != kv_lens.shape[0]:
-        raise RuntimeError(f"block_table {tuple(block_table.shape)}, query_starts {tuple(query_starts.shape)} and kv_lens "
+    if not (block_table.dtype is torch.int32 and query_starts.dtype is torch.int32 and kv_lens.dtype is torch.int32
+            and block_table.get_device() == dev and query_starts.get_device() == dev and kv_lens.get_device() == dev):
+        raise RuntimeError("block_table, query_starts and kv_lens must be int32 tensors on the cache's device")
+    table = block_table.shape
+    batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    if len(table) != 2 or table[0] != batch or query_starts.shape != (batch + 1,):
+        raise RuntimeError(f"block_table {tuple(table)}, query_starts {tuple(query_starts.shape)} and kv_lens "
                            f"{tuple(kv_lens.shape)} must be [B, pages], [B + 1] and [B]")
-    batch, width = block_table.shape
-    if width > 1 and block_table.stride(1) != 1 or batch > 1 and block_table.stride(0) < width \
-            or not query_starts.is_contiguous() or not kv_lens.is_contiguous():
+    width = table[1]
+    stride, inner = block_table.stride()
+    if batch <= 1:
+        stride = width
+    if (width > 1 and inner != 1) or stride < width or not (query_starts.is_contiguous() and kv_lens.is_contiguous()):
         raise RuntimeError("block_table rows, query_starts and kv_lens must be packed")
-    if max_query_len is None:
+    if max_query_len is None or max_query_len > tokens:
         max_query_len = tokens
-    stride = block_table.stride(0) if batch > 1 else width
-    return _PagedBatch(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(),
-                       kv_lens.data_ptr(), pages, hkv, page_size, d, stride, width, batch, tokens,
-                       max_query_len), dev, hkv, d
+    pages, hkv, page_size, d = shape
+    packed = _pack_paged_batch(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(),
+                               kv_lens.data_ptr(), pages, hkv, page_size, d, stride, width, batch, tokens, max_query_len)
+    return packed, dev, batch, hkv, page_size, d, width, max_query_len
 
 
 def _paged_rows(t, name, tokens, d, dev, dtype):
-    """Element stride between the tokens of `t` [tokens, heads, d], whose heads and columns are packed."""
-    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and t.device == dev and t.dtype == dtype):
-        raise RuntimeError(f"{name} must be a 3-dimensional {dtype} tensor on {dev}")
+    """(heads, element stride between the tokens) of `t` [tokens, heads, d], whose heads and columns are packed."""
+    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and t.get_device() == dev and t.dtype is dtype):
+        raise RuntimeError(f"{name} must be a 3-dimensional {dtype} tensor on the cache's device")
     n, h, dd = t.shape
-    st = t.stride()
-    if n != tokens or dd != d or d > 1 and st[2] != 1 or h > 1 and st[1] != d:
+    token, head, column = t.stride()
+    if n != tokens or dd != d or (d > 1 and column != 1) or (h > 1 and head != d):
         raise RuntimeError(f"{name} must be [{tokens}, heads, {d}] with packed heads, got shape {tuple(t.shape)} "
-                           f"and strides {st}")
-    return st[0] if n > 1 else h * d
+                           f"and strides {t.stride()}")
+    return h, token if n > 1 else h * d
 
 
-_PAGED_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+def _paged_call(fn, batch, args, dev):
+    cur = _current_device()
+    if cur == dev:
+        rc = fn(batch, args, _raw_stream(dev))
+    else:
+        torch.cuda.set_device(dev)
+        try:
+            rc = fn(batch, args, _raw_stream(dev))
+        finally:
+            torch.cuda.set_device(cur)
+    _check(rc)
 
 
 def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, max_query_len=None, q=None,
@@ -699,31 +704,27 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     Extends torch.cat((past, new)) of torch_int/models/opt.py:113-116."""
     if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _PAGED_DTYPES:
         raise RuntimeError("k must be a 3-dimensional float32, float16, bfloat16 or int8 tensor")
-    n = k.shape[0]
-    batch, dev, hkv, d = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
-    ld_k = _paged_rows(k, "k", n, d, dev, k.dtype)
-    ld_v = _paged_rows(v, "v", n, d, dev, k.dtype)
-    if k.shape[1] != hkv or v.shape[1] != hkv:
-        raise RuntimeError(f"k has {k.shape[1]} and v {v.shape[1]} heads, the cache {hkv}")
-    q_ptr = out_ptr = rot_ptr = None
-    ld_q = hq = rows = rd = 0
+    n, dtype = k.shape[0], k.dtype
+    batch, dev, _, hkv, _, d, _, _ = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
+    hk, ld_k = _paged_rows(k, "k", n, d, dev, dtype)
+    hv, ld_v = _paged_rows(v, "v", n, d, dev, dtype)
+    if hk != hkv or hv != hkv:
+        raise RuntimeError(f"k has {hk} and v {hv} heads, the cache {hkv}")
+    q_ptr = out_ptr = rot_ptr = ld_q = hq = rows = rd = 0
     out = None
     if q is not None:
-        ld_q = _paged_rows(q, "q", n, d, dev, k.dtype)
-        hq = q.shape[1]
-        out = torch.empty((n, hq, d), dtype=torch.int8, device=dev)
+        hq, ld_q = _paged_rows(q, "q", n, d, dev, dtype)
+        out = q.new_empty((n, hq, d), dtype=torch.int8)
         q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
     if rotary is not None:
-        if not (isinstance(rotary, torch.Tensor) and rotary.dtype == torch.float32 and rotary.device == dev
+        if not (isinstance(rotary, torch.Tensor) and rotary.dtype is torch.float32 and rotary.get_device() == dev
                 and rotary.dim() == 2 and rotary.is_contiguous()):
-            raise RuntimeError(f"rotary must be a contiguous float32 tensor [positions, rotary_dim] on {dev}")
+            raise RuntimeError("rotary must be a contiguous float32 tensor [positions, rotary_dim] on the cache's device")
         rows, rd = rotary.shape
         rot_ptr = rotary.data_ptr()
-    args = _PagedAppendArgs(q_ptr, k.data_ptr(), v.data_ptr(), ld_q, ld_k, ld_v, hq, rot_ptr, rows, rd, out_ptr,
-                            q_alpha, k_alpha, v_alpha, _PAGED_DTYPES[k.dtype], 1 if interleaved else 0)
-    with _on_device(dev):
-        rc = _c_paged_append(batch, args, _stream_ptr(dev))
-    _check(rc)
+    args = _pack_paged_append(q_ptr, k.data_ptr(), v.data_ptr(), ld_q, ld_k, ld_v, hq, rot_ptr, rows, rd, out_ptr,
+                              q_alpha, k_alpha, v_alpha, _PAGED_DTYPES[dtype], 1 if interleaved else 0)
+    _paged_call(_c_paged_append, batch, args, dev)
     return out
 
 
@@ -739,26 +740,25 @@ def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     Replaces the attention core of torch_int/models/opt.py:131-181 for sequences of unequal lengths."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise RuntimeError("q must be a 3-dimensional int8 tensor")
-    n, hq, _ = q.shape
-    batch, dev, hkv, d = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
-    ld_q = _paged_rows(q, "q", n, d, dev, torch.int8)
+    n = q.shape[0]
+    batch, dev, b, hkv, page_size, d, width, max_q = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens,
+                                                                  n, max_query_len)
+    hq, ld_q = _paged_rows(q, "q", n, d, dev, torch.int8)
     if max_kv_len is None:
-        max_kv_len = batch.table_width * batch.page_size
+        max_kv_len = width * page_size
     if out is None:
-        out = torch.empty((n, hq, d), dtype=out_dtype, device=dev)
-    elif not (isinstance(out, torch.Tensor) and out.device == dev and out.shape == q.shape and out.is_contiguous()):
-        raise RuntimeError(f"out must be a contiguous {tuple(q.shape)} tensor on {dev}")
+        out = q.new_empty((n, hq, d), dtype=out_dtype)
+    elif not (isinstance(out, torch.Tensor) and out.get_device() == dev and out.shape == q.shape and out.is_contiguous()):
+        raise RuntimeError(f"out must be a contiguous {tuple(q.shape)} tensor on the cache's device")
     kind = _PAGED_DTYPES.get(out.dtype, 0)
     if kind == 0:
         raise RuntimeError(f"the context must be int8, float16 or bfloat16, not {out.dtype}")
-    need = _c_paged_workspace(batch.batch, n, hq, hkv, d, batch.max_query_len, max_kv_len)
+    need = _c_paged_workspace(b, n, hq, hkv, d, max_q, max_kv_len)
     # scratch of this call alone: the allocator orders its reuse by stream, and a captured graph keeps its own
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    args = _PagedAttentionArgs(q.data_ptr(), ld_q, hq, max_kv_len, out.data_ptr(), ws.data_ptr() if need else None,
-                               need, alpha_qk, alpha_pv, kind)
-    with _on_device(dev):
-        rc = _c_paged_attention(batch, args, _stream_ptr(dev))
-    _check(rc)
+    ws = q.new_empty(need) if need else None
+    args = _pack_paged_attention(q.data_ptr(), ld_q, hq, max_kv_len, out.data_ptr(), ws.data_ptr() if need else 0,
+                                 need, alpha_qk, alpha_pv, kind)
+    _paged_call(_c_paged_attention, batch, args, dev)
     return out
 
 
