@@ -5,20 +5,25 @@
 //
 // paged_rows_kernel serves sequences with few query rows per key head (rows = new tokens x group), decode
 // above all: it is bound by the bytes of the cache, 2 * head_dim per key and key head, each read once.
-//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; its warps take 16 keys at a time.
+//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; a warp takes 32 keys at a time, as two groups of
+//     16 (a group lies in one page, in consecutive bytes).
 //   * Scores transposed, S^T = K . Q^T (m16n8k32 s8, keys as rows, queries as the 8 columns), so that a single
 //     query row wastes 7 of 8 columns and not 15 of 16 rows; the context likewise, O^T = V^T . P^T (m16n8k16
 //     fp16).  The columns of a dot product may be taken in any order as long as both operands agree, and so may
-//     the rows of O^T: the order is chosen so that each lane loads its fragments straight from the pools with
-//     16-byte (V of 64- and 80-wide heads: 8-byte) loads that use every sector they touch; no shared memory
-//     and no barrier in the loop, one group of keys is in flight while the one before is multiplied.
+//     the rows of O^T: the order is chosen so that a lane's fragments are 16-byte pieces of a row (V of 64- and
+//     80-wide heads: 8).
+//   * Groups come through a queue of the warp in shared memory (cp.async, whole lines, no registers and no barrier of
+//     the block), in an order of pieces that makes the fragments' reads free of bank conflicts.  The loop is bound
+//     by the latency of its own instructions, not by the depth of the queue (2, 3 and 4 groups in flight: the same):
+//     hence 32 keys a step, whose two halves overlap.
 //   * int8 values become fp16 exactly (byte + 1152 as the low bits of 1024.., minus 1152).
 //   * Running maximum in the log2 domain per warp, raised only when a score exceeds it by more than 8 (a vote,
 //     no reduction, in the common case); probabilities are 2^(s - max + 7) <= 2^15, split into two fp16 numbers
 //     (p = hi + lo, 22 bits) whose products are summed in fp32: the tensor cores have room for the second
 //     product because the loop waits for memory.
-// The keys are split over CTAs; each writes its unnormalised context, maximum and sum in fp32, and
-// paged_combine_kernel joins them in a fixed order (no atomics: results do not depend on timing).
+// The keys are split over CTAs.  Up to MAX_CLUSTER splits are a cluster, whose CTAs join their partial results
+// through distributed shared memory: one launch, no workspace.  More splits write them in fp32 to a workspace and
+// paged_combine_kernel joins them.  Both in a fixed order, without atomics: results do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,13 +33,17 @@
 #include "grid_dependency.cuh"
 #include "paged.h"
 #include "paged_attention.cuh"
+#define TI_PTX_EXTERNAL_STATUS 1
+#include "sm100_ptx.cuh"
 
 namespace ti {
 namespace {
 
 constexpr int ROWS_WARPS = 4;
 constexpr int ROWS_THREADS = ROWS_WARPS * 32;
-constexpr int MAX_CHUNK = 32 * ROWS_WARPS * 16;  // a lane holds the page of one of its warp's key groups
+constexpr int STAGES = 2;           // steps of a warp in shared memory: one in flight, one in use
+constexpr int STEP = 32;            // keys of a step: two groups of 16
+constexpr int MAX_CLUSTER = 8;
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -54,41 +63,30 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Streaming loads: every byte of the cache is read by one warp only.
-__device__ __forceinline__ uint4 ld_stream16(const int8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy_async16(uint32_t dst, const int8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ld_stream8(const int8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+// 2^x to about 2 ulp.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ uint32_t ld_stream4(const int8_t* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // The columns of a row that lane `a` (= lane % 4) holds for a dot product: 16 bytes of each 64, and 4 bytes of
 // the last 16 of an 80-wide row.
 template <int D>
 struct DotRow {
-  static constexpr int WORDS = D / 16;
   static constexpr int STEPS = (D + 31) / 32;
   uint32_t w[2 * STEPS];
+  __device__ __forceinline__ void put(const uint4& x, int i) { w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w; }
   __device__ __forceinline__ void load(const int8_t* row, int a) {
-    const uint4 x = ld_stream16(row + a * 16);
-    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    if constexpr (D == 128) {
-      const uint4 y = ld_stream16(row + 64 + a * 16);
-      w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
-    } else if constexpr (D == 80) {
-      w[4] = ld_stream4(row + 64 + a * 4);
-      w[5] = 0;
-    }
+    put(__ldg(reinterpret_cast<const uint4*>(row + a * 16)), 0);
+    if constexpr (D == 128) put(__ldg(reinterpret_cast<const uint4*>(row + 64 + a * 16)), 1);
+    if constexpr (D == 80) w[4] = __ldg(reinterpret_cast<const uint32_t*>(row + 64 + a * 4)), w[5] = 0;
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -102,16 +100,6 @@ template <int D>
 struct ValueRow {
   static constexpr int WORDS = D == 128 ? 4 : D == 80 ? 3 : 2;
   uint32_t w[WORDS];
-  __device__ __forceinline__ void load(const int8_t* row, int g) {
-    if constexpr (D == 128) {
-      const uint4 x = ld_stream16(row + g * 16);
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else {
-      const uint2 x = ld_stream8(row + g * 8);
-      w[0] = x.x, w[1] = x.y;
-      if constexpr (D == 80) w[2] = __ldg(reinterpret_cast<const uint16_t*>(row + 64 + g * 2));
-    }
-  }
 };
 // Column of the even row of output tile i (its other row is the next column).
 template <int D>
@@ -120,6 +108,57 @@ __device__ __forceinline__ int value_column(int g, int i) {
   return i < 4 ? g * 8 + 2 * i : 64 + 2 * g;
 }
 
+// A group of 16 keys in shared memory: rows of D bytes as in the pools, K then V.  The 16-byte pieces of a 128-byte
+// row are stored in another order, so that the eight lanes that read at a time find their pieces in different banks:
+// K (rows g, g + 1, pieces a) exchanges the halves of odd rows, V (rows 2a, pieces g) xors with the row's bits 1, 2;
+// of the 64-byte rows of V four lanes share two rows' banks.
+template <int D>
+struct Group {
+  static constexpr int V = 16 * D, BYTES = 2 * V;
+  static __device__ __forceinline__ int key_piece(int row, int c) { return D == 128 ? c ^ ((row & 1) << 2) : c; }
+  static __device__ __forceinline__ int value_piece(int row, int c) {
+    return D == 128 ? c ^ (row & 6) : D == 64 ? c ^ ((row >> 1) & 3) : c;
+  }
+  // kp, vp: first key's row in the pools
+  static __device__ __forceinline__ void fetch(uint32_t at, const int8_t* kp, const int8_t* vp, int lane) {
+    constexpr int PIECES = D / 16;  // of a row
+#pragma unroll
+    for (int i = 0; i < (D + 31) / 32; ++i) {
+      const int n = i * 32 + lane;  // 16 * PIECES in all
+      if (D % 32 != 0 && n >= D) continue;
+      const int row = n / PIECES, c = n - row * PIECES;
+      copy_async16(at + row * D + key_piece(row, c) * 16, kp + n * 16);
+      copy_async16(at + V + row * D + value_piece(row, c) * 16, vp + n * 16);
+    }
+  }
+  static __device__ __forceinline__ void keys(const uint8_t* s, int lane, DotRow<D> (&kr)[2]) {
+    const int a = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = (lane >> 2) + 8 * i;
+      kr[i].put(*reinterpret_cast<const uint4*>(s + row * D + key_piece(row, a) * 16), 0);
+      if constexpr (D == 128) kr[i].put(*reinterpret_cast<const uint4*>(s + row * D + key_piece(row, 4 + a) * 16), 1);
+      if constexpr (D == 80) kr[i].w[4] = *reinterpret_cast<const uint32_t*>(s + row * D + 64 + a * 4), kr[i].w[5] = 0;
+    }
+  }
+  static __device__ __forceinline__ void values(const uint8_t* s, int lane, ValueRow<D> (&vr)[4]) {
+    const int g = lane >> 2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = 2 * (lane & 3) + (j & 1) + 8 * (j >> 1);
+      const uint8_t* r = s + V + row * D;
+      if constexpr (D == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(r + value_piece(row, g) * 16);
+        vr[j].w[0] = x.x, vr[j].w[1] = x.y, vr[j].w[2] = x.z, vr[j].w[3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(r + value_piece(row, g >> 1) * 16 + (g & 1) * 8);
+        vr[j].w[0] = x.x, vr[j].w[1] = x.y;
+        if constexpr (D == 80) vr[j].w[2] = *reinterpret_cast<const uint16_t*>(r + 64 + g * 2);
+      }
+    }
+  }
+};
+
 // Bytes (lo, hi byte pairs of two rows) -> fp16 pairs, exactly.
 __device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t sel) {
   const uint32_t h = __byte_perm(x, 0x64646464u, sel);  // 1024 + (byte ^ 0x80)
@@ -127,25 +166,79 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// CTAs of paged_rows_kernel an SM holds: registers (147 per thread of 128-wide heads) and the queues' 64 KB.
+__host__ __device__ constexpr int rows_ctas_per_sm(int head_dim, int nt) {
+  return head_dim == 128 ? (nt == 1 ? 3 : 2) : (nt == 1 ? 4 : 3);
+}
+
+// Shared memory of a rows CTA: the warps' queues; when they are empty, the warps' contexts and what they join to.
 template <int D, int NT>
-__global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kernel(const PagedAttnParams p) {
-  constexpr int R = 8 * NT;
+struct RowsSmem {
+  static constexpr int R = 8 * NT, LDO = D + 4;
+  static constexpr int STAGE = 2 * Group<D>::BYTES, QUEUE = ROWS_WARPS * STAGES * STAGE;
+  static constexpr int JOINED = ROWS_WARPS * R * LDO * 4;          // fp32 [R][D]
+  static constexpr int BYTES = QUEUE > JOINED + R * D * 4 ? QUEUE : JOINED + R * D * 4;
+};
+
+__device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ float2 ld_cluster8(uint32_t addr) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr) : "memory");
+  return x;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_rows_kernel(const PagedAttnParams p) {
+  using SM = RowsSmem<D, NT>;
+  constexpr int R = SM::R, LDO = SM::LDO;
   constexpr int MT = D / 16;  // 16-row tiles of O^T
-  constexpr int LDO = D + 4;
-  __shared__ __align__(16) float s_o[ROWS_WARPS][R][LDO];
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[ROWS_WARPS][R], s_l[ROWS_WARPS][R];
+  __shared__ float2 s_ml[R];
+  float(*s_o)[R][LDO] = reinterpret_cast<float(*)[R][LDO]>(smem);
+  float* s_join = reinterpret_cast<float*>(smem + SM::JOINED);
   const PagedView& v = p.view;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, a = lane & 3;
   const int b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles, h = blockIdx.y, split = blockIdx.x;
   PagedSeq s;
   grid_dep_launch();
-  if (!paged_sequence(v, b, p.max_kv_len, &s)) return;
+  grid_dep_wait();
+  if (!paged_sequence(v, b, p.max_kv_len, &s)) return;  // (returns before the keys are looked at: a whole cluster's)
   const int G = p.group, rows = s.T * G, r0 = rt * R;
   if (r0 >= rows || rows > p.rows_below) return;
   const int past = s.L - s.T;
   const PagedSplits sp = paged_splits(past + (min(r0 + R, rows) - 1) / G + 1, p.chunk);
-  if (split >= sp.n) return;
-  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, sp.keys);
+  if (split >= sp.n && (!p.cluster || sp.n == 1)) return;
+  const int k0 = min(split * p.chunk, sp.keys), k1 = min(k0 + p.chunk, sp.keys);
+
+  // this warp's steps: keys k0 + (warp + ROWS_WARPS * i) * STEP, i < cnt; lane n knows the page of group n of 32
+  const int steps = (k1 - k0 + STEP - 1) / STEP;
+  const int cnt = steps > warp ? (steps - warp + ROWS_WARPS - 1) / ROWS_WARPS : 0;
+  const uint32_t queue = smem_u32(smem) + warp * STAGES * SM::STAGE;
+  int my_page = 0;
+  auto fetch = [&](int i) {  // in order, every i < cnt once
+    if (i < cnt) {
+      if ((i & 15) == 0) {
+        const int key = k0 + (warp + ROWS_WARPS * (i + (lane >> 1))) * STEP + (lane & 1) * 16;
+        my_page = key < k1 ? max(0, paged_page(v, b, key >> v.page_shift)) : 0;
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = k0 + (warp + ROWS_WARPS * i) * STEP + n * 16;
+        const long long page = __shfl_sync(0xffffffffu, my_page, (i & 15) * 2 + n);
+        const long long at = (((page * v.kv_heads + h) << v.page_shift) + (key & ((1 << v.page_shift) - 1))) * D;
+        if (key < k1)
+          Group<D>::fetch(queue + (i % STAGES) * SM::STAGE + n * Group<D>::BYTES, v.k_pages + at, v.v_pages + at, lane);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
   // query fragments and limits
   DotRow<D> qf[NT];
@@ -160,12 +253,6 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
   }
   const int lim_min = past + r0 / G;
 
-  // this warp's key groups: k0 + (warp + ROWS_WARPS * i) * 16, i < cnt; lane i knows the page of group i
-  const int groups = (k1 - k0 + 15) >> 4;
-  const int cnt = groups > warp ? (groups - warp + ROWS_WARPS - 1) / ROWS_WARPS : 0;
-  int my_page = 0;
-  if (lane < cnt) my_page = max(0, paged_page(v, b, (k0 + (warp + ROWS_WARPS * lane) * 16) >> v.page_shift));
-
   float o[NT][MT][4];
   float m[NT][2], l[NT][2];
 #pragma unroll
@@ -177,62 +264,58 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
     m[n][0] = m[n][1] = -1e30f;
     l[n][0] = l[n][1] = 0.f;
   }
-  DotRow<D> kr[2];
-  ValueRow<D> vr[4];
-  auto fetch = [&](int i) {
-    const int key = k0 + (warp + ROWS_WARPS * i) * 16;
-    const long long page = __shfl_sync(0xffffffffu, my_page, i);
-    const long long at = (((page * v.kv_heads + h) << v.page_shift) + (key & ((1 << v.page_shift) - 1))) * D;
-    const int8_t* kp = v.k_pages + at;
-    const int8_t* vp = v.v_pages + at;
-    kr[0].load(kp + g * D, a);
-    kr[1].load(kp + (g + 8) * D, a);
-    vr[0].load(vp + (2 * a) * D, g);
-    vr[1].load(vp + (2 * a + 1) * D, g);
-    vr[2].load(vp + (2 * a + 8) * D, g);
-    vr[3].load(vp + (2 * a + 9) * D, g);
-  };
-  if (cnt > 0) fetch(0);
 #pragma unroll 1
   for (int i = 0; i < cnt; ++i) {
-    const int key = k0 + (warp + ROWS_WARPS * i) * 16;
-    int acc[NT][4];
+    const int key = k0 + (warp + ROWS_WARPS * i) * STEP;
+    const uint8_t* stage = smem + (warp * STAGES + i % STAGES) * SM::STAGE;
+    copy_wait<STAGES - 2>();
+    __syncwarp();  // step i has landed, and every lane is done with the one whose place the next fetch takes
+    fetch(i + STAGES - 1);
+    // scores (log2 domain): columns 2a, 2a + 1 are queries, rows g, g + 8 keys of a group
+    float sc[2][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+    for (int u = 0; u < 2; ++u) {
+      DotRow<D> kr[2];
+      Group<D>::keys(stage + u * Group<D>::BYTES, lane, kr);
 #pragma unroll
-      for (int k = 0; k < DotRow<D>::STEPS; ++k) {
-        const uint32_t fa[4] = {kr[0].w[2 * k], kr[1].w[2 * k], kr[0].w[2 * k + 1], kr[1].w[2 * k + 1]};
-        mma_s8(acc[n], fa, qf[n].w[2 * k], qf[n].w[2 * k + 1]);
+      for (int n = 0; n < NT; ++n) {
+        int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < DotRow<D>::STEPS; ++k) {
+          const uint32_t fa[4] = {kr[0].w[2 * k], kr[1].w[2 * k], kr[0].w[2 * k + 1], kr[1].w[2 * k + 1]};
+          mma_s8(acc, fa, qf[n].w[2 * k], qf[n].w[2 * k + 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[u][n][c] = static_cast<float>(acc[c]) * p.scale_log2;
       }
     }
-    ValueRow<D> vc[4];
+    if (key + STEP - 1 > lim_min) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vc[j] = vr[j];
-    if (i + 1 < cnt) fetch(i + 1);
-    // scores (log2 domain): columns 2a, 2a + 1 are queries, rows g, g + 8 keys
-    float sc[NT][4];
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key + u * 16 + g + (c >> 1) * 8 > lim[n][c & 1]) sc[u][n][c] = -INFINITY;
+    }
+    float top[NT][2];
     bool raise = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sc[n][c] = static_cast<float>(acc[n][c]) * p.scale_log2;
-      if (key + 15 > lim_min) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (key + g + (c >> 1) * 8 > lim[n][c & 1]) sc[n][c] = -INFINITY;
+      for (int c = 0; c < 2; ++c) {
+        top[n][c] = fmaxf(fmaxf(sc[0][n][c], sc[0][n][c + 2]), fmaxf(sc[1][n][c], sc[1][n][c + 2]));
+        raise |= top[n][c] > m[n][c] + 8.f;
       }
-      raise |= fmaxf(sc[n][0], sc[n][2]) > m[n][0] + 8.f || fmaxf(sc[n][1], sc[n][3]) > m[n][1] + 8.f;
-    }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(m[n][c], fmaxf(sc[n][c], sc[n][c + 2]));
+          float mx = fmaxf(m[n][c], top[n][c]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float corr = exp2f(m[n][c] - mx);
+          const float corr = ex2(m[n][c] - mx);
           m[n][c] = mx;
           l[n][c] *= corr;
 #pragma unroll
@@ -243,44 +326,55 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
         }
       }
     }
-    uint32_t ph[NT][2], pl[NT][2];
+    uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float e[4];
+      const float base[2] = {7.f - m[n][0], 7.f - m[n][1]};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        e[c] = exp2f(sc[n][c] - m[n][c & 1] + 7.f);
-        l[n][c & 1] += e[c];
-      }
+      for (int u = 0; u < 2; ++u) {
+        float e[4];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const __half2 hi = __floats2half2_rn(e[2 * c], e[2 * c + 1]);
-        const float2 back = __half22float2(hi);
-        const __half2 lo = __floats2half2_rn(e[2 * c] - back.x, e[2 * c + 1] - back.y);
-        ph[n][c] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-        pl[n][c] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
+        for (int c = 0; c < 4; ++c) {
+          e[c] = ex2(sc[u][n][c] + base[c & 1]);
+          l[n][c & 1] += e[c];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const __half2 hi = __floats2half2_rn(e[2 * c], e[2 * c + 1]);
+          const float2 back = __half22float2(hi);
+          const __half2 lo = __floats2half2_rn(e[2 * c] - back.x, e[2 * c + 1] - back.y);
+          ph[u][n][c] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+          pl[u][n][c] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
+        }
       }
     }
 #pragma unroll
-    for (int w = 0; w < ValueRow<D>::WORDS; ++w) {
+    for (int u = 0; u < 2; ++u) {
+      ValueRow<D> vc[4];
+      Group<D>::values(stage + u * Group<D>::BYTES, lane, vc);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = 2 * w + half;
-        if (t >= MT) continue;
-        const uint32_t pick = half ? 0x7362u : 0x5140u;
-        const uint32_t x01 = __byte_perm(vc[0].w[w], vc[1].w[w], pick) ^ 0x80808080u;
-        const uint32_t x23 = __byte_perm(vc[2].w[w], vc[3].w[w], pick) ^ 0x80808080u;
-        const uint32_t fa[4] = {halves_of(x01, 0x4140), halves_of(x01, 0x4342), halves_of(x23, 0x4140),
-                                halves_of(x23, 0x4342)};
+      for (int w = 0; w < ValueRow<D>::WORDS; ++w) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_f16(o[n][t], fa, ph[n][0], ph[n][1]);
-          mma_f16(o[n][t], fa, pl[n][0], pl[n][1]);
+        for (int half = 0; half < 2; ++half) {
+          const int t = 2 * w + half;
+          if (t >= MT) continue;
+          const uint32_t pick = half ? 0x7362u : 0x5140u;
+          const uint32_t x01 = __byte_perm(vc[0].w[w], vc[1].w[w], pick) ^ 0x80808080u;
+          const uint32_t x23 = __byte_perm(vc[2].w[w], vc[3].w[w], pick) ^ 0x80808080u;
+          const uint32_t fa[4] = {halves_of(x01, 0x4140), halves_of(x01, 0x4342), halves_of(x23, 0x4140),
+                                  halves_of(x23, 0x4342)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(o[n][t], fa, ph[u][n][0], ph[u][n][1]);
+            mma_f16(o[n][t], fa, pl[u][n][0], pl[u][n][1]);
+          }
         }
       }
     }
   }
   // ---- join the warps: each had its own maximum
+  copy_wait<0>();
+  __syncthreads();  // the queues are empty: their memory is used again
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -292,15 +386,17 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
         s_m[warp][r] = m[n][c];
         s_l[warp][r] = l[n][c];
       }
+      if (r0 + r < rows) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-        *reinterpret_cast<float2*>(&s_o[warp][r][value_column<D>(g, t)]) = make_float2(o[n][t][c], o[n][t][c + 2]);
+        for (int t = 0; t < MT; ++t)
+          *reinterpret_cast<float2*>(&s_o[warp][r][value_column<D>(g, t)]) = make_float2(o[n][t][c], o[n][t][c + 2]);
+      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < R * (D / 4); i += ROWS_THREADS) {
+  const int work = min(R, rows - r0) * (D / 4);
+  for (int i = threadIdx.x; i < work; i += ROWS_THREADS) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
-    if (row >= rows) break;
     float mx = s_m[0][r];
 #pragma unroll
     for (int w = 1; w < ROWS_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
@@ -319,20 +415,57 @@ __global__ void __launch_bounds__(ROWS_THREADS, NT == 1 ? 4 : 2) paged_rows_kern
     const long long at = static_cast<long long>(s.q0 + row / G) * p.q_heads + h * G + row % G;
     if (sp.n == 1) {
       paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
+    } else if (p.cluster) {
+      *reinterpret_cast<float4*>(s_join + r * D + d) = x;
+      if (d == 0) s_ml[r] = make_float2(mx, sum);
     } else {
       *reinterpret_cast<float4*>(p.part_o + (at * p.max_splits + split) * D + d) = x;
       if (d == 0) p.part_ml[at * p.max_splits + split] = make_float2(mx, sum);
     }
   }
+  if (sp.n == 1 || !p.cluster) return;
+  // ---- join the splits of the cluster (rank = split), each CTA a part of the rows and columns
+  cluster_sync_all();
+  const uint32_t join_at = smem_u32(s_join), ml_at = smem_u32(s_ml);
+  for (int i = split * ROWS_THREADS + threadIdx.x; i < work; i += static_cast<int>(gridDim.x) * ROWS_THREADS) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
+    float mx = -1e30f, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 ml[MAX_CLUSTER];
+    float4 y[MAX_CLUSTER];
+#pragma unroll
+    for (int c = 0; c < MAX_CLUSTER; ++c) {
+      if (c >= sp.n) continue;
+      ml[c] = ld_cluster8(mapa_shared(ml_at + r * 8, c));
+      y[c] = ld_cluster16(mapa_shared(join_at + (r * D + d) * 4, c));
+      mx = fmaxf(mx, ml[c].x);
+    }
+#pragma unroll
+    for (int c = 0; c < MAX_CLUSTER; ++c) {
+      if (c >= sp.n) continue;
+      const float f = exp2f(ml[c].x - mx);
+      sum += f * ml[c].y;
+      x.x += f * y[c].x;
+      x.y += f * y[c].y;
+      x.z += f * y[c].z;
+      x.w += f * y[c].w;
+    }
+    const long long at = static_cast<long long>(s.q0 + row / G) * p.q_heads + h * G + row % G;
+    paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
+  }
+  cluster_sync_all();  // the others may still read this CTA's part
 }
 
-// One warp per (token, query head): joins the partial contexts of the row's splits, in order.
+// One block per (token, query head): joins the partial contexts of the row's splits, every fourth one in a warp (a
+// single warp took 14 us for 56 splits, most of it waiting for its loads), then the warps'.
 template <int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParams p, int few_rows, int many_rows,
                                                             int many_chunk) {
+  __shared__ float4 s_x[4][32];
+  __shared__ float s_m[4], s_l[4];
   const PagedView& v = p.view;
-  const int b = blockIdx.y, lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5);  // (token, head) of the sequence
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x;  // (token, head) of the sequence
   PagedSeq s;
   const bool ok = paged_sequence(v, b, p.max_kv_len, &s);
   grid_dep_wait();
@@ -344,34 +477,71 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
   const int R = many ? many_rows : few_rows;
   const int r = t * G + head % G;
   const PagedSplits sp = paged_splits(s.L - s.T + (min((r / R + 1) * R, rows) - 1) / G + 1, many ? many_chunk : p.chunk);
-  if (sp.n == 1) return;  // written by the attention kernel
+  if (sp.n == 1 || (!many && p.cluster)) return;  // written by the attention kernel
   const long long at = static_cast<long long>(s.q0 + t) * p.q_heads + head;
   const float2* ml = p.part_ml + at * p.max_splits;
-  float mx = -1e30f;
-  for (int i = lane; i < sp.n; i += 32) mx = fmaxf(mx, ml[i].x);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
   const int d = lane * 4;
   const bool mine = d < D;
-  const float* po = p.part_o + at * p.max_splits * D + d;
-  float sum = 0.f;
+  const float* po = p.part_o + at * p.max_splits * D + (mine ? d : 0);
+  float mx = -1e30f, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < sp.n; ++i) {
-    const float2 e = ml[i];
-    const float f = exp2f(e.x - mx);
-    const float4 y = mine ? *reinterpret_cast<const float4*>(po + static_cast<long long>(i) * D) : x;
-    sum += f * e.y;
+  constexpr int BATCH = 8;  // splits whose loads are in flight together
+  for (int i0 = warp; i0 < sp.n; i0 += 4 * BATCH) {
+    float2 e[BATCH];
+    float4 y[BATCH];
+    float top = mx;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = min(i0 + 4 * k, sp.n - 1);
+      e[k] = ml[i];
+      y[k] = *reinterpret_cast<const float4*>(po + static_cast<long long>(i) * D);
+      if (i0 + 4 * k >= sp.n) e[k] = make_float2(-1e30f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) top = fmaxf(top, e[k].x);
+    const float corr = exp2f(mx - top);
+    mx = top;
+    sum *= corr;
+    x.x *= corr;
+    x.y *= corr;
+    x.z *= corr;
+    x.w *= corr;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const float f = i0 + 4 * k < sp.n ? exp2f(e[k].x - mx) : 0.f;
+      sum += f * e[k].y;
+      x.x += f * y[k].x;
+      x.y += f * y[k].y;
+      x.z += f * y[k].z;
+      x.w += f * y[k].w;
+    }
+  }
+  s_x[warp][lane] = x;
+  if (lane == 0) {
+    s_m[warp] = mx;
+    s_l[warp] = sum;
+  }
+  __syncthreads();
+  if (warp != 0 || !mine) return;
+  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  sum = 0.f;
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = exp2f(s_m[w] - mx);
+    const float4 y = s_x[w][lane];
+    sum += f * s_l[w];
     x.x += f * y.x;
     x.y += f * y.y;
     x.z += f * y.z;
     x.w += f * y.w;
   }
-  if (mine) paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
+  paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
 }
 
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
 constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
+constexpr int MIN_CHUNK = 512, MAX_CHUNK = 2048;  // keys of a split of paged_rows_kernel
 
 // How a call is cut.  Sequences with at most `few` rows per key head are served by paged_rows_kernel, the others by
 // paged_tiles_kernel; a kernel is left out where the bounds show that no sequence needs it.
@@ -379,14 +549,16 @@ struct Plan {
   bool rows, tiles;
   int few;
   int nt, row_tiles, chunk, row_splits;  // rows kernel: 8-row tiles of a CTA, CTAs of a sequence, keys of a split
+  bool cluster;                          // the splits of the rows kernel are a cluster
   PagedTilePlan tile;
-  int splits;                            // the larger number of splits: stride of the partial results
+  int splits;                            // most splits that go through the workspace: stride of the partial results
 };
 
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 int64_t div_up(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
-Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int64_t max_query_len, int64_t max_kv_len) {
+Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int head_dim, int64_t max_query_len,
+               int64_t max_kv_len) {
   Plan pl = {};
   const int64_t rows = max_query_len * group;
   pl.few = group > TILE_ROWS ? 0x7FFFFFFF : FEW_ROWS;
@@ -396,17 +568,21 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   pl.rows = !pl.tiles || shortest * group <= pl.few;
   pl.splits = 1;
   if (pl.rows) {
-    // Enough CTAs for about two rounds on all SMs when every sequence has the maximum length, so that shorter ones
-    // still fill them, but not below 128 keys (a CTA's fixed costs) nor above MAX_CHUNK.
     const int64_t most = rows < pl.few ? rows : pl.few;
     pl.nt = most <= 8 ? 1 : 2;
     pl.row_tiles = static_cast<int>(div_up(most, 8 * pl.nt));
-    const int64_t units = batch * kv_heads * pl.row_tiles, want = PAGED_SMS * (pl.nt == 1 ? 4 : 2) * 2;
-    int64_t chunk = round_up(div_up(max_kv_len, units >= want ? 1 : div_up(want, units)), 16);
-    chunk = chunk < 128 ? 128 : chunk > MAX_CHUNK ? MAX_CHUNK : chunk;
+    // One CTA per unit where that fills the SMs, in pieces of at most MAX_CHUNK keys (sequences of unequal lengths:
+    // 64 contexts of up to 8192 keys took 94 us in pieces of 1024 to 2048 keys, 102 in whole).  Otherwise as many pieces
+    // as fill the SMs once (two contexts of 131072 keys: 82 us so, 110 with a third more pieces), of at least MIN_CHUNK
+    // keys (one context of 500 keys: 7.6 us in one piece, 8.8 in four).
+    const int64_t units = batch * kv_heads * pl.row_tiles, slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt);
+    int64_t chunk = units >= slots ? MAX_CHUNK : round_up(div_up(max_kv_len, slots / units), STEP);
+    if (chunk < MIN_CHUNK) chunk = MIN_CHUNK;
     pl.chunk = static_cast<int>(chunk);
     pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
-    pl.splits = pl.row_splits;
+    // a cluster holds its CTAs until the last one is done: only where all of them run at once
+    pl.cluster = pl.row_splits > 1 && pl.row_splits <= MAX_CLUSTER && units * pl.row_splits <= slots;
+    if (!pl.cluster) pl.splits = pl.row_splits;
   }
   if (pl.tiles) {
     pl.tile.tokens_per_tile = static_cast<int>(TILE_ROWS / group);
@@ -421,15 +597,41 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   return pl;
 }
 
+template <int D, int NT>
+cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaStream_t stream) {
+  auto kernel = paged_rows_kernel<D, NT>;
+  constexpr int smem = RowsSmem<D, NT>::BYTES;
+  static PagedOncePerDevice once;
+  const cudaError_t e = once.run([kernel] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
+                     static_cast<unsigned>(b.batch * pl.row_tiles));
+  cfg.blockDim = dim3(ROWS_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(pl.row_splits);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.cluster ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int D>
 int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaStream_t stream) {
   if (pl.rows) {
-    const dim3 grid(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
-                    static_cast<unsigned>(b.batch * pl.row_tiles));
-    if (pl.nt == 1)
-      paged_rows_kernel<D, 1><<<grid, ROWS_THREADS, 0, stream>>>(p);
-    else
-      paged_rows_kernel<D, 2><<<grid, ROWS_THREADS, 0, stream>>>(p);
+    const cudaError_t e = pl.nt == 1 ? launch_rows<D, 1>(b, p, pl, stream) : launch_rows<D, 2>(b, p, pl, stream);
+    if (e != cudaSuccess) {
+      set_error("paged_attention launch failed: %s", cudaGetErrorString(e));
+      return TI_E_CUDA;
+    }
   }
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && pl.tiles) {
@@ -438,7 +640,10 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
   }
   if (e == cudaSuccess && pl.splits > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(div_up(b.max_query_len * p.q_heads, 4)), static_cast<unsigned>(b.batch));
+    // only the rows of few-row sequences have partial results where the tile kernel does not split
+    const int64_t few_tokens = pl.few / p.group;
+    const int64_t tokens = pl.tiles && pl.tile.splits == 1 && few_tokens < b.max_query_len ? few_tokens : b.max_query_len;
+    cfg.gridDim = dim3(static_cast<unsigned>(tokens * p.q_heads), static_cast<unsigned>(b.batch));
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -461,7 +666,7 @@ int64_t paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q
                                         int64_t head_dim, int64_t max_query_len, int64_t max_kv_len) {
   if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_query_len <= 0 || max_kv_len <= 0) return 0;
   if (max_query_len > tokens) max_query_len = tokens;
-  const Plan pl = make_plan(batch, tokens, q_heads / kv_heads, kv_heads, max_query_len, max_kv_len);
+  const Plan pl = make_plan(batch, tokens, q_heads / kv_heads, kv_heads, static_cast<int>(head_dim), max_query_len, max_kv_len);
   return pl.splits == 1 ? 0 : tokens * q_heads * pl.splits * (head_dim * 4 + 8);
 }
 
@@ -494,7 +699,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
     return TI_E_INVALID;
   }
   const int64_t group = a.q_heads / b.kv_heads;
-  const Plan pl = make_plan(b.batch, b.tokens, group, b.kv_heads, b.max_query_len, a.max_kv_len);
+  const Plan pl = make_plan(b.batch, b.tokens, group, b.kv_heads, static_cast<int>(b.head_dim), b.max_query_len, a.max_kv_len);
   if (b.batch * static_cast<int64_t>(pl.row_tiles) > 65535 || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
     set_error("paged_attention: batch %lld x %lld new tokens is too large for one call", (long long)b.batch,
               (long long)b.max_query_len);
@@ -526,6 +731,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   p.row_tiles = pl.row_tiles;
   p.chunk = pl.chunk;
   p.max_splits = pl.splits;
+  p.cluster = pl.cluster;
   p.rows_below = pl.tiles ? pl.few : 0x7FFFFFFF;
   if (!pl.rows) p.rows_below = 0;
   p.part_o = static_cast<float*>(a.workspace);

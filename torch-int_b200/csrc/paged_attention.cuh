@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "paged_device.cuh"
 
 namespace ti {
@@ -21,13 +23,32 @@ struct PagedAttnParams {
   int out_kind;       // 1 fp16, 2 bf16, 3 int8
   int row_tiles;      // of the largest sequence
   int chunk;          // keys of a split, a multiple of 16
-  int max_splits;
+  int max_splits;     // stride of the partial results
+  int cluster;        // the splits of the rows kernel are a cluster and need no partial results
   int rows_below;     // sequences with at most this many rows belong to the rows kernel, the others to the tile kernel
   float* part_o;      // [tokens * q_heads][max_splits][head_dim], unnormalised
   float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
 };
 
 constexpr int PAGED_SMS = 148;
+
+// Runs a kernel's set-up (function attributes) the first time it is launched on a device: a call of its own costs
+// about as much as a launch.
+class PagedOncePerDevice {
+ public:
+  template <typename F>
+  cudaError_t run(F&& f) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done_.load(std::memory_order_acquire) >> dev & 1))) return e;
+    e = f();
+    if (e == cudaSuccess && dev < 64) done_.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<unsigned long long> done_{0};
+};
 
 // How the tile kernel (paged_attention_sm100.cu) cuts the work.
 struct PagedTilePlan {

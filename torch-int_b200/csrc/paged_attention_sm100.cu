@@ -763,17 +763,18 @@ int launch(const PagedBatch& b, const PagedAttnParams& a, const PagedTilePlan& p
       !make_operand_map(&tv, b.v_pages, D, b.page_size, b.kv_heads, b.num_pages, D, page_bytes, b.kv_heads * page_bytes, box))
     return TI_E_CUDA;
   auto kernel = paged_tiles_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES);
-  if (e == cudaSuccess) {
+  static PagedOncePerDevice once;
+  cudaError_t e = once.run([kernel] {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES);
+    if (err != cudaSuccess) return err;
     // the warpgroups' register split has to fit what the block is launched with, or the kernel would wait for good
-    static const int regs = [kernel] {
-      cudaFuncAttributes fa;
-      return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : 0;
-    }();
-    if (regs * THREADS < REGS_SOFTMAX * 512 + REGS_CONVERT * 128 + REGS_OTHER * 128) {
-      set_error("paged_attention: the kernel was built with %d registers per thread, too few for its warpgroups", regs);
-      return TI_E_CUDA;
-    }
+    cudaFuncAttributes fa;
+    const cudaError_t got = cudaFuncGetAttributes(&fa, kernel);
+    if (got != cudaSuccess) return got;
+    return fa.numRegs * THREADS < REGS_SOFTMAX * 512 + REGS_CONVERT * 128 + REGS_OTHER * 128 ? cudaErrorLaunchOutOfResources
+                                                                                            : cudaSuccess;
+  });
+  if (e == cudaSuccess) {
     // persistent: one CTA per SM, or per work item where the bounds allow fewer
     const int64_t most = (b.batch < MAX_SEQS ? b.batch : MAX_SEQS) * static_cast<int64_t>(plan.pairs) * plan.splits * b.kv_heads;
     const unsigned grid = static_cast<unsigned>(most < PAGED_SMS ? most : PAGED_SMS);
