@@ -5,11 +5,13 @@
 // Every product, sum and difference is rounded to fp32 by itself (no contraction), so that the int8 results
 // are defined bit by bit whatever the compiler does; int8 -> int8 with alpha = 1 and no rotation is a copy.
 //
-// Bound by bytes: (q_heads + 2 kv_heads) * head_dim * (size of the input + 1) per token, each touched once.
-// A thread owns 16 columns of one head of one token: two runs of 8 (the two halves of 8 rotated pairs, or
-// 16 neighbours), so that every access is 8 to 32 contiguous bytes and a pool row of a head is written by
-// neighbouring lanes.  UNITS of them are loaded before the first is used.  The page lookup of a token is
-// done once per block, into shared memory.
+// Bound by bytes: (q_heads + 2 kv_heads) * head_dim * (size of the input + 1) per token, each touched once.  A unit is
+// 16 columns of one head of one token: two runs of 8 (the two halves of 8 rotated pairs, or 16 neighbours), so that
+// every access is 8 to 32 contiguous bytes and a pool row of a head is written by neighbouring lanes.  A block takes a
+// range of a sequence's units, cut so that few tokens still spread over many blocks and many tokens do not pay a
+// block's fixed latency (lengths, then pages, then data) too often; the page lookups of its tokens go through shared
+// memory.  What hides the latencies is occupancy: two units in flight per thread at 64 registers move more than four
+// at 93 did.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -17,6 +19,7 @@
 #include <stdint.h>
 
 #include "gemm_i8.h"
+#include "grid_dependency.cuh"
 #include "paged.h"
 #include "paged_device.cuh"
 
@@ -24,7 +27,9 @@ namespace ti {
 namespace {
 
 constexpr int APPEND_THREADS = 256;
-constexpr int APPEND_MAX_TOKENS = 32;  // tokens of a block at most (page lookups in shared memory)
+constexpr int PAGED_APPEND_BLOCKS = 4 * 148;
+constexpr int APPEND_MAX_UNITS = 2048;                          // of a block
+constexpr int APPEND_MAX_TOKENS = APPEND_MAX_UNITS / (2 * 4) + 2;  // it can touch: a token has at least 8 units
 
 struct AppendParams {
   PagedView view;
@@ -36,7 +41,7 @@ struct AppendParams {
   int8_t* q_out;
   int q_heads;
   int units_per_token;     // (q_heads + 2 kv_heads) * D / 16
-  int tokens_per_block;
+  int units_per_block;
 };
 
 // Four floats -> four int8 in one word: rne, saturated; NaN -> 0.
@@ -99,126 +104,147 @@ struct Raw8<int8_t> {
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const AppendParams p) {
+// COPY: int8 rows stored as they are.
+template <typename T, int D, bool COPY>
+__global__ void __launch_bounds__(APPEND_THREADS, COPY ? 6 : 4) paged_append_kernel(const AppendParams p) {
   constexpr int PIECES = D / 16;
-  constexpr int UNITS = sizeof(T) == 4 ? 2 : 4;  // units a thread has in flight
-  __shared__ int s_row[APPEND_MAX_TOKENS];       // page * page_size + row, -1: nothing to store
-  __shared__ int s_pos[APPEND_MAX_TOKENS];
+  constexpr int UNITS = COPY ? 4 : 2;             // units a thread has in flight
+  __shared__ int s_row[APPEND_MAX_TOKENS];        // page * page_size + row, -1: nothing to store
   const PagedView& v = p.view;
-  const int b = blockIdx.y, t0 = blockIdx.x * p.tokens_per_block;
+  const int b = blockIdx.y, tid = threadIdx.x;
+  grid_dep_launch();
+  grid_dep_wait();
   PagedSeq s;
   if (!paged_sequence(v, b, INT_MAX, &s)) return;
   if (s.L < s.T) {  // the new tokens are part of the keys
-    if (threadIdx.x == 0) atomicCAS(v.status, 0, static_cast<int>(TI_ERR_PAGED_LENGTHS));
+    if (tid == 0) atomicCAS(v.status, 0, static_cast<int>(TI_ERR_PAGED_LENGTHS));
     return;
   }
-  const int nt = min(p.tokens_per_block, s.T - t0);
-  if (nt <= 0) return;
-  if (static_cast<int>(threadIdx.x) < nt) {
-    const int pos = s.L - s.T + t0 + threadIdx.x;
+  const int upt = p.units_per_token;
+  const long long u0 = static_cast<long long>(blockIdx.x) * p.units_per_block;
+  if (u0 >= static_cast<long long>(s.T) * upt) return;
+  const int t0 = static_cast<int>(u0 / upt), skip = static_cast<int>(u0 - static_cast<long long>(t0) * upt);
+  const int nt = min((skip + p.units_per_block + upt - 1) / upt, s.T - t0);
+  const int pos0 = s.L - s.T + t0;
+  for (int i = tid; i < nt; i += APPEND_THREADS) {
+    const int pos = pos0 + i;
     const int page = paged_page(v, b, pos >> v.page_shift);
     int row = page < 0 ? -1 : (page << v.page_shift) + (pos & ((1 << v.page_shift) - 1));
     if (p.rotary != nullptr && pos >= p.rotary_rows) {
       atomicCAS(v.status, 0, static_cast<int>(TI_ERR_PAGED_LENGTHS));
       row = -1;
     }
-    s_row[threadIdx.x] = row;
-    s_pos[threadIdx.x] = pos;
+    s_row[i] = row;
   }
   __syncthreads();
-  const int total = nt * p.units_per_token;
+  const int end = min(skip + p.units_per_block, nt * upt);
   const int hk = v.kv_heads, rd = p.rotary_dim;
   const long long token0 = s.q0 + t0;
-  for (int base = threadIdx.x; base < total; base += APPEND_THREADS * UNITS) {
+  for (int base = skip + tid; base < end; base += APPEND_THREADS * UNITS) {
     Raw8<T> lo[UNITS], hi[UNITS];
-    int tok[UNITS], which[UNITS], head[UNITS], off0[UNITS], off1[UNITS], pair0[UNITS];
+    uint4 whole[UNITS];
+    int8_t* dst[UNITS];
+    int tok[UNITS], piece[UNITS], cls[UNITS];  // cls: 0 q, 1 k, 2 v, -1 none
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int idx = base + u * APPEND_THREADS;
-      which[u] = -1;
-      if (idx >= total) continue;
-      const int t = idx / p.units_per_token;
-      const int rest = idx - t * p.units_per_token;
-      if (s_row[t] < 0) continue;
-      const int hh = rest / PIECES, piece = rest - hh * PIECES;
-      which[u] = hh < p.q_heads ? 0 : hh < p.q_heads + hk ? 1 : 2;
-      head[u] = hh - (which[u] == 0 ? 0 : which[u] == 1 ? p.q_heads : p.q_heads + hk);
+      cls[u] = -1;
+      if (idx >= end) continue;
+      const int t = idx / upt, rest = idx - t * upt, row = s_row[t];
+      if (row < 0) continue;
+      const int hh = rest / PIECES;
+      piece[u] = rest - hh * PIECES;
       tok[u] = t;
-      const bool rotated = which[u] < 2 && piece * 16 < rd;
-      pair0[u] = rotated ? piece * 8 : -1;
-      const bool halves = rotated && !p.interleaved;
-      off0[u] = halves ? piece * 8 : piece * 16;
-      off1[u] = halves ? rd / 2 + piece * 8 : piece * 16 + 8;
-      const T* src = static_cast<const T*>(p.src[which[u]]) + (token0 + t) * p.ld[which[u]] + head[u] * D;
-      lo[u].load(src + off0[u]);
-      hi[u].load(src + off1[u]);
+      int head;
+      if (hh < p.q_heads) {
+        cls[u] = 0;
+        head = hh;
+        dst[u] = p.q_out + ((token0 + t) * p.q_heads + head) * D;
+      } else {
+        cls[u] = hh < p.q_heads + hk ? 1 : 2;
+        head = hh - p.q_heads - (cls[u] == 2 ? hk : 0);
+        const long long page = row >> v.page_shift;
+        const int in_page = row & ((1 << v.page_shift) - 1);
+        dst[u] = (cls[u] == 1 ? v.k_pages : v.v_pages) + ((((page * hk) + head) << v.page_shift) + in_page) * D;
+      }
+      const T* src = static_cast<const T*>(p.src[cls[u]]) + (token0 + t) * p.ld[cls[u]] + head * D;
+      if constexpr (COPY) {
+        whole[u] = __ldg(reinterpret_cast<const uint4*>(src + piece[u] * 16));
+      } else {
+        const bool halves = cls[u] < 2 && piece[u] * 16 < rd && !p.interleaved;
+        lo[u].load(src + (halves ? piece[u] * 8 : piece[u] * 16));
+        hi[u].load(src + (halves ? rd / 2 + piece[u] * 8 : piece[u] * 16 + 8));
+      }
     }
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      if (which[u] < 0) continue;
-      float x[8], y[8];
-      lo[u].get(x);
-      hi[u].get(y);
-      if (pair0[u] >= 0) {
-        const float* c = p.rotary + static_cast<long long>(s_pos[tok[u]]) * rd + pair0[u];
-        const float* sn = c + rd / 2;
-        float cs[8], ss[8];
-        *reinterpret_cast<float4*>(cs) = __ldg(reinterpret_cast<const float4*>(c));
-        *reinterpret_cast<float4*>(cs + 4) = __ldg(reinterpret_cast<const float4*>(c) + 1);
-        *reinterpret_cast<float4*>(ss) = __ldg(reinterpret_cast<const float4*>(sn));
-        *reinterpret_cast<float4*>(ss + 4) = __ldg(reinterpret_cast<const float4*>(sn) + 1);
-        auto turn = [](float& a, float& d, float co, float si) {
-          const float a1 = __fsub_rn(__fmul_rn(a, co), __fmul_rn(d, si));
-          d = __fadd_rn(__fmul_rn(d, co), __fmul_rn(a, si));
-          a = a1;
-        };
-        if (p.interleaved) {
+      if (cls[u] < 0) continue;
+      if constexpr (COPY) {
+        *reinterpret_cast<uint4*>(dst[u] + piece[u] * 16) = whole[u];
+      } else {
+        float x[8], y[8];
+        lo[u].get(x);
+        hi[u].get(y);
+        const bool rotated = cls[u] < 2 && piece[u] * 16 < rd;
+        if (rotated) {
+          const float* c = p.rotary + static_cast<long long>(pos0 + tok[u]) * rd + piece[u] * 8;
+          const float* sn = c + rd / 2;
+          auto turn = [](float& a, float& d, float co, float si) {
+            const float a1 = __fsub_rn(__fmul_rn(a, co), __fmul_rn(d, si));
+            d = __fadd_rn(__fmul_rn(d, co), __fmul_rn(a, si));
+            a = a1;
+          };
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            turn(x[2 * i], x[2 * i + 1], cs[i], ss[i]);
-            turn(y[2 * i], y[2 * i + 1], cs[4 + i], ss[4 + i]);
+          for (int q = 0; q < 2; ++q) {
+            const float4 cs = __ldg(reinterpret_cast<const float4*>(c) + q), ss = __ldg(reinterpret_cast<const float4*>(sn) + q);
+            if (p.interleaved) {
+              float(&z)[8] = q == 0 ? x : y;
+              turn(z[0], z[1], cs.x, ss.x);
+              turn(z[2], z[3], cs.y, ss.y);
+              turn(z[4], z[5], cs.z, ss.z);
+              turn(z[6], z[7], cs.w, ss.w);
+            } else {
+              turn(x[4 * q], y[4 * q], cs.x, ss.x);
+              turn(x[4 * q + 1], y[4 * q + 1], cs.y, ss.y);
+              turn(x[4 * q + 2], y[4 * q + 2], cs.z, ss.z);
+              turn(x[4 * q + 3], y[4 * q + 3], cs.w, ss.w);
+            }
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) turn(x[i], y[i], cs[i], ss[i]);
         }
-      }
-      const float al = p.alpha[which[u]];
+        const float al = p.alpha[cls[u]];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = __fmul_rn(x[i], al);
-        y[i] = __fmul_rn(y[i], al);
-      }
-      const uint2 a = make_uint2(quantise4(x[0], x[1], x[2], x[3]), quantise4(x[4], x[5], x[6], x[7]));
-      const uint2 d = make_uint2(quantise4(y[0], y[1], y[2], y[3]), quantise4(y[4], y[5], y[6], y[7]));
-      int8_t* dst;
-      if (which[u] == 0) {
-        dst = p.q_out + ((token0 + tok[u]) * p.q_heads + head[u]) * D;
-      } else {
-        const int row = s_row[tok[u]];
-        const long long page = row >> v.page_shift;
-        const int in_page = row & ((1 << v.page_shift) - 1);
-        dst = (which[u] == 1 ? v.k_pages : v.v_pages) + ((((page * hk) + head[u]) << v.page_shift) + in_page) * D;
-      }
-      if (off1[u] == off0[u] + 8) {
-        *reinterpret_cast<uint4*>(dst + off0[u]) = make_uint4(a.x, a.y, d.x, d.y);
-      } else {
-        *reinterpret_cast<uint2*>(dst + off0[u]) = a;
-        *reinterpret_cast<uint2*>(dst + off1[u]) = d;
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __fmul_rn(x[i], al);
+          y[i] = __fmul_rn(y[i], al);
+        }
+        const uint2 a = make_uint2(quantise4(x[0], x[1], x[2], x[3]), quantise4(x[4], x[5], x[6], x[7]));
+        const uint2 d = make_uint2(quantise4(y[0], y[1], y[2], y[3]), quantise4(y[4], y[5], y[6], y[7]));
+        if (rotated && !p.interleaved) {
+          *reinterpret_cast<uint2*>(dst[u] + piece[u] * 8) = a;
+          *reinterpret_cast<uint2*>(dst[u] + rd / 2 + piece[u] * 8) = d;
+        } else {
+          *reinterpret_cast<uint4*>(dst[u] + piece[u] * 16) = make_uint4(a.x, a.y, d.x, d.y);
+        }
       }
     }
   }
 }
 
-template <typename T>
-void launch_append(int head_dim, dim3 grid, const AppendParams& p, cudaStream_t stream) {
-  if (head_dim == 128)
-    paged_append_kernel<T, 128><<<grid, APPEND_THREADS, 0, stream>>>(p);
-  else if (head_dim == 80)
-    paged_append_kernel<T, 80><<<grid, APPEND_THREADS, 0, stream>>>(p);
-  else
-    paged_append_kernel<T, 64><<<grid, APPEND_THREADS, 0, stream>>>(p);
+// Launched as a programmatic dependent: the launch overlaps the end of the kernel before it, which it waits for.
+template <typename T, bool COPY>
+cudaError_t launch_append(int head_dim, dim3 grid, const AppendParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(APPEND_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (head_dim == 128) return cudaLaunchKernelEx(&cfg, paged_append_kernel<T, 128, COPY>, p);
+  if (head_dim == 80) return cudaLaunchKernelEx(&cfg, paged_append_kernel<T, 80, COPY>, p);
+  return cudaLaunchKernelEx(&cfg, paged_append_kernel<T, 64, COPY>, p);
 }
 
 }  // namespace
@@ -308,21 +334,24 @@ int paged_append(const PagedBatch& b, const PagedAppend& a, cudaStream_t stream)
   p.q_out = a.q_out;
   p.q_heads = static_cast<int>(q_heads);
   p.units_per_token = static_cast<int>((q_heads + 2 * b.kv_heads) * (b.head_dim / 16));
-  // about two rounds of the loop per block, at most APPEND_MAX_TOKENS page lookups
+  // Blocks of up to APPEND_MAX_UNITS units, smaller ones where the tokens would not fill four blocks per SM.
   const int64_t max_q = b.max_query_len < b.tokens ? b.max_query_len : b.tokens;
-  int64_t per_block = 2048 / p.units_per_token;
-  per_block = per_block < 1 ? 1 : per_block > APPEND_MAX_TOKENS ? APPEND_MAX_TOKENS : per_block;
-  p.tokens_per_block = static_cast<int>(per_block < max_q ? per_block : max_q);
-  const dim3 grid(static_cast<unsigned>((max_q + p.tokens_per_block - 1) / p.tokens_per_block),
-                  static_cast<unsigned>(b.batch));
-  const int d = static_cast<int>(b.head_dim);
-  switch (a.dtype) {
-    case 0: launch_append<float>(d, grid, p, stream); break;
-    case 1: launch_append<__half>(d, grid, p, stream); break;
-    case 2: launch_append<__nv_bfloat16>(d, grid, p, stream); break;
-    default: launch_append<int8_t>(d, grid, p, stream); break;
+  int64_t units = b.tokens * p.units_per_token / (PAGED_APPEND_BLOCKS * APPEND_THREADS) * APPEND_THREADS;
+  units = units < APPEND_THREADS ? APPEND_THREADS : units > APPEND_MAX_UNITS ? APPEND_MAX_UNITS : units;
+  p.units_per_block = static_cast<int>(units);
+  const int64_t blocks = (max_q * p.units_per_token + units - 1) / units;
+  if (blocks > 0x7FFFFFFF) {
+    set_error("paged_append: too many new tokens for one call");
+    return TI_E_INVALID;
   }
-  const cudaError_t e = cudaGetLastError();
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(b.batch));
+  const int d = static_cast<int>(b.head_dim);
+  const bool copy = a.dtype == 3 && a.rotary == nullptr && a.k_alpha == 1.f && a.v_alpha == 1.f && (!a.q || a.q_alpha == 1.f);
+  const cudaError_t e = a.dtype == 0   ? launch_append<float, false>(d, grid, p, stream)
+                        : a.dtype == 1 ? launch_append<__half, false>(d, grid, p, stream)
+                        : a.dtype == 2 ? launch_append<__nv_bfloat16, false>(d, grid, p, stream)
+                        : copy         ? launch_append<int8_t, true>(d, grid, p, stream)
+                                       : launch_append<int8_t, false>(d, grid, p, stream);
   if (e != cudaSuccess) {
     set_error("paged_append launch failed: %s", cudaGetErrorString(e));
     return TI_E_CUDA;
