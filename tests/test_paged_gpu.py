@@ -450,3 +450,59 @@ def test_refusals_on_gpu_tensors(cuda_ops):
     with pytest.raises(RuntimeError, match="v must be"):
         C.paged_append(k, k.half(), *index_args(b))
     assert C.device_status() == 0
+
+
+# ----------------------------------------------------------------------------------------------- in the model
+@pytest.fixture(scope="module")
+def opt_model():
+    from torch_int.models.opt import Int8OPTConfig
+    from torch_int.models.random_init import random_int8_opt
+    cfg = Int8OPTConfig(vocab_size=512, hidden_size=256, num_hidden_layers=2, ffn_dim=512, num_attention_heads=4,
+                        max_position_embeddings=512)
+    return random_int8_opt(cfg, seed=5, device="cuda")
+
+
+def prompts_of(*lens):
+    g = torch.Generator().manual_seed(9)
+    return [torch.randint(2, 512, (n,), generator=g).cuda() for n in lens]
+
+
+def close(a, b, tol=2e-2):
+    """A batch and a sequence alone may be cut differently, so an int8 context may differ by a unit where it lies near a
+    half: by the operator's bound (2^-11 of a spread of about 10 units, to both sides) in at most 2 * 2^-11 * 10 = 1 % of
+    the 256 columns, 2.6 of them.  A unit is 1 / (10 * sqrt(256)) = 0.6 % of a context of 10 units per column, so a
+    layer's attention output is off by about sqrt(2.6) * 0.6 % = 1 %, two layers' by 1.4 % at most of the residual."""
+    return float((a - b).norm() / b.norm()) < tol
+
+
+def test_model_batch_agrees_with_its_sequences_alone(cuda_ops, opt_model):
+    prompts = prompts_of(200, 1, 37, 64)
+    cache = opt_model.new_paged_cache(40)
+    seqs = [cache.open() for _ in prompts]
+    got = opt_model.forward_paged(torch.cat(prompts), cache, cache.step(seqs, [len(p) for p in prompts]))
+    for i, p in enumerate(prompts):
+        alone = opt_model.new_paged_cache(20, page_size=32)
+        want = opt_model.forward_paged(p, alone, alone.step([alone.open()], [len(p)]))
+        assert close(got[i:i + 1], want)
+    # a chunk for one sequence, single tokens for two others
+    new = prompts_of(90, 1, 1)
+    step = cache.step([seqs[3], seqs[0], seqs[1]], [90, 1, 1])
+    got = opt_model.forward_paged(torch.cat(new), cache, step)
+    for i, s in enumerate((3, 0, 1)):
+        alone = opt_model.new_paged_cache(30)
+        h = alone.open()
+        opt_model.forward_paged(prompts[s], alone, alone.step([h], [len(prompts[s])]))
+        want = opt_model.forward_paged(new[i], alone, alone.step([h], [len(new[i])]))
+        assert close(got[i:i + 1], want)
+    assert cuda_ops.device_status() == 0
+
+
+def test_model_generates_the_same_eagerly_and_from_a_graph(cuda_ops, opt_model):
+    prompts = prompts_of(30, 5, 100)
+    eager = opt_model.generate_paged(prompts, 12, use_cuda_graph=False)
+    graph = opt_model.generate_paged(prompts, 12)
+    assert all(torch.equal(a, b) for a, b in zip(eager, graph))
+    assert [len(x) for x in graph] == [42, 17, 112] and all(torch.equal(x[:len(p)], p) for x, p in zip(graph, prompts))
+    one = opt_model.generate_paged(prompts[:1], 1)
+    assert torch.equal(one[0], graph[0][:31])
+    assert cuda_ops.device_status() == 0

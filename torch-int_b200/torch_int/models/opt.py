@@ -43,6 +43,7 @@ from ..nn.bmm import BMM_S8T_S8N_F32T, BMM_S8T_S8N_S8T
 from ..nn.fused import LayerNormQ
 from ..nn.linear import W8A8B8O8Linear, W8A8B8O8LinearReLU, W8A8BFP32OFP32Linear
 from .kv_cache import StaticInt8KVCache
+from .paged_cache import PagedInt8KVCache, PagedStep
 from .tensor_parallel import TensorParallel
 
 
@@ -191,10 +192,11 @@ class Int8OPTAttention(nn.Module):
     @torch.no_grad()
     def forward_fused(self, hidden_int8, cache: Optional[StaticInt8KVCache], layer_idx: int, past_len: int,
                       mask: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, b0: int = 0,
-                      context_only: bool = False, decode: bool = False):
+                      context_only: bool = False, decode: bool = False, paged: Optional[PagedStep] = None):
         """int8 [B,T,E] -> int32 partial sums of out_proj [B*T, E] (this rank's input
         slice; bias and scale are applied after the reduction over the ranks).  `out`:
-        optional destination; `b0`: index of the first of these sequences in the cache."""
+        optional destination; `b0`: index of the first of these sequences in the cache.
+        With `paged`, hidden_int8 is [1,N,E], the step's new tokens, and `cache` a PagedInt8KVCache."""
         bsz, tgt_len, _ = hidden_int8.shape
         hl, d, el = self.local_heads, self.head_dim, self.local_dim
         x2d = hidden_int8.view(-1, self.embed_dim)
@@ -208,6 +210,21 @@ class Int8OPTAttention(nn.Module):
         C.gemm_i8_ex(x2d, w, qkv, bias, epilogue=C.EPI_S8_BIAS_S8_VEC, m=tokens, n=3 * el, k=self.embed_dim,
                      lda=self.embed_dim, ldb=self.embed_dim, ldc=3 * el, alpha_vec=alpha_vec, beta_vec=beta_vec)
         ld = 3 * el
+        if paged is not None:
+            heads = qkv[:tokens].view(tokens, 3 * hl, d)
+            kp, vp = cache.k_pages[layer_idx], cache.v_pages[layer_idx]
+            C.paged_append(heads[:, hl:2 * hl], heads[:, 2 * hl:], kp, vp, paged.block_table, paged.query_starts,
+                           paged.kv_lens, max_query_len=paged.max_query_len)
+            # pv_bmm's scale counts probabilities in units of 1/127
+            ctx = C.paged_attention(heads[:, :hl], kp, vp, paged.block_table, paged.query_starts, paged.kv_lens,
+                                    alpha_qk=self.qk_bmm._alpha(), alpha_pv=127.0 * self.pv_bmm._alpha(),
+                                    max_query_len=paged.max_query_len, max_kv_len=paged.max_kv_len).view(1, tokens, el)
+            if context_only:
+                return ctx
+            acc = out if out is not None else torch.empty((tokens, self.embed_dim), dtype=torch.int32, device=ctx.device)
+            C.gemm_i8_ex(ctx.view(tokens, el), self.out_proj.weight, acc, epilogue=C.EPI_S32_RAW, m=tokens,
+                         n=self.embed_dim, k=el, lda=el, ldb=el, ldc=self.embed_dim)
+            return acc
         if decode:
             # one new token per sequence: append + scores + softmax + context in one kernel that reads
             # the position from device memory (no per-step host parameters: CUDA-graph friendly)
@@ -352,7 +369,7 @@ class Int8OPTDecoderLayer(nn.Module):
     # ------------------------------------------------------------------ fast path
     @torch.no_grad()
     def forward_fused(self, residual, hidden_int8, cache, layer_idx, past_len, mask, next_ln: Optional[LayerNormQ],
-                      decode: bool = False, inplace: bool = False):
+                      decode: bool = False, inplace: bool = False, paged: Optional[PagedStep] = None):
         """residual fp [B,T,E], hidden_int8 = LayerNormQ(residual) -> (new residual,
         int8 input of the next layer or None).  `next_ln` is the next layer's
         self_attn_layer_norm (None after the last layer).  `inplace`: the caller owns `residual` and lets
@@ -366,7 +383,7 @@ class Int8OPTDecoderLayer(nn.Module):
             # only normalises and quantises: the int32 products never travel through HBM.
             e = self.embed_dim
             res2d = residual.view(-1, e)
-            ctx = attn.forward_fused(hidden_int8, cache, layer_idx, past_len, mask, context_only=True)
+            ctx = attn.forward_fused(hidden_int8, cache, layer_idx, past_len, mask, context_only=True, paged=paged)
             ctx2d = ctx.view(-1, attn.local_dim)
             C.gemm_i8_ex(ctx2d, attn.out_proj.weight, res2d, attn.out_proj.bias, epilogue=C.EPI_F32_BIAS_F32_ACC,
                          m=res2d.shape[0], n=e, k=attn.local_dim, lda=attn.local_dim, ldb=attn.local_dim, ldc=e,
@@ -380,7 +397,7 @@ class Int8OPTDecoderLayer(nn.Module):
             if next_ln is None:
                 return residual, None
             return residual, C.layernorm_q(residual, next_ln.weight, next_ln.bias, next_ln.eps)
-        acc = attn.forward_fused(hidden_int8, cache, layer_idx, past_len, mask, decode=decode)
+        acc = attn.forward_fused(hidden_int8, cache, layer_idx, past_len, mask, decode=decode, paged=paged)
         acc = self.tp.all_reduce_int32(acc)
         ln = self.final_layer_norm
         residual, h8 = C.dq_add_layernorm_q_bias(acc.view(shape), attn.out_proj._scalar("a"), attn.out_proj.bias,
@@ -694,6 +711,39 @@ class Int8OPTDecoder(nn.Module):
             residual = self.project_out(residual)
         return residual
 
+    def new_paged_cache(self, num_pages: int, page_size: int = 16, device=None) -> PagedInt8KVCache:
+        """Pools of `num_pages` pages of `page_size` positions per layer, for sequences of any lengths."""
+        attn = self.layers[0].self_attn
+        device = device if device is not None else self.embed_tokens.weight.device
+        return PagedInt8KVCache(len(self.layers), num_pages, attn.local_heads, attn.head_dim, device, page_size)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.LongTensor, cache: PagedInt8KVCache, step: PagedStep) -> torch.Tensor:
+        """The new tokens [N] of a step, sequence after sequence, on top of what the paged cache holds of their
+        sequences: last hidden state [N, proj].  Prompts, chunks of prompts and single tokens may be mixed.  All
+        position dependent values are read on the device, so a step of fixed sizes can be captured in a CUDA graph
+        and replayed (PagedStep.advance).  The attention does not round its probabilities to int8 (see
+        C.paged_attention), so results differ from the static cache's in their last digits."""
+        n = tokens.shape[0]
+        hidden = self.embed_tokens(tokens)
+        if self.project_in is not None:
+            hidden = self.project_in(hidden)
+        hidden = hidden + nn.functional.embedding(step.positions + self.embed_positions.offset, self.embed_positions.weight)
+        hidden = hidden.view(1, n, -1)
+        residual = hidden.to(self._stream_dtype(hidden)).contiguous()
+        first = self.layers[0].self_attn_layer_norm
+        h8 = C.layernorm_q(residual, first.weight, first.bias, first.eps)
+        nl = len(self.layers)
+        for i, layer in enumerate(self.layers):
+            next_ln = self.layers[i + 1].self_attn_layer_norm if i + 1 < nl else None
+            residual, h8 = layer.forward_fused(residual, h8, cache, i, None, None, next_ln, inplace=True, paged=step)
+        residual = residual.to(hidden.dtype).view(n, -1)
+        if self.final_layer_norm is not None:
+            residual = self.final_layer_norm(residual)
+        if self.project_out is not None:
+            residual = self.project_out(residual)
+        return residual
+
     @torch.no_grad()
     def forward(self, input_ids: torch.LongTensor, attention_mask: Optional[torch.Tensor] = None,
                 past_key_values: Optional[StaticInt8KVCache] = None, use_cache: bool = False,
@@ -925,3 +975,64 @@ class Int8OPTForCausalLM(nn.Module):
                 nxt = self.decode_step(nxt, cache).argmax(dim=-1, keepdim=True)
         tokens.append(nxt)
         return torch.cat(tokens, dim=1)
+
+    def new_paged_cache(self, num_pages, page_size=16, device=None):
+        return self.model.decoder.new_paged_cache(num_pages, page_size, device)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens, cache: PagedInt8KVCache, step: PagedStep, last_token_only=True):
+        """Logits [B, vocab] after the last new token of each sequence of the step, or [N, vocab] of all of them."""
+        hidden = self.model.decoder.forward_paged(tokens, cache, step)
+        if last_token_only:
+            hidden = hidden.index_select(0, step.last)
+        return self._logits(hidden)
+
+    @torch.no_grad()
+    def generate_paged(self, prompts: List[torch.Tensor], max_new_tokens: int, cache: Optional[PagedInt8KVCache] = None,
+                       use_cuda_graph: Optional[bool] = None) -> List[torch.Tensor]:
+        """Greedy decoding of prompts of unequal lengths as one batch over a paged cache: all prompts in one step, then
+        one token per sequence and step (replayed from a CUDA graph by default on a single GPU).  Returns each prompt
+        with its new tokens.  A cache that is passed in may hold other sequences; it is left as it was."""
+        dec = self.model.decoder
+        if not prompts or max_new_tokens < 1:
+            raise ValueError("generate_paged needs a prompt and at least one new token")
+        device = dec.embed_tokens.weight.device
+        lens = [int(p.numel()) for p in prompts]
+        if min(lens) < 1:
+            raise ValueError("every prompt needs at least one token")
+        if cache is None:
+            cache = self.new_paged_cache(sum(-(-(n + max_new_tokens - 1) // 16) for n in lens))
+        if use_cuda_graph is None:
+            use_cuda_graph = dec.tp.size == 1
+        seqs = [cache.open() for _ in lens]
+        try:
+            cache.reserve({s: n + max_new_tokens - 1 for s, n in zip(seqs, lens)})
+            flat = torch.cat([p.reshape(-1) for p in prompts]).to(device)
+            nxt = self.forward_paged(flat, cache, cache.step(seqs, lens)).argmax(dim=-1)
+            new = [nxt]
+            left = max_new_tokens - 1
+            if left > 0:
+                step = cache.step(seqs, [1] * len(seqs))
+                step.max_kv_len = max(lens) + max_new_tokens - 1  # the bound of every later step as well
+                nxt = self.forward_paged(nxt, cache, step).argmax(dim=-1)
+                new.append(nxt)
+                left -= 1
+            if left > 0 and use_cuda_graph:
+                static = nxt.clone()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    step.advance()
+                    static.copy_(self.forward_paged(static, cache, step).argmax(dim=-1))
+                for _ in range(left):
+                    graph.replay()
+                    new.append(static.clone())
+            else:
+                for _ in range(left):
+                    step.advance()
+                    nxt = self.forward_paged(nxt, cache, step).argmax(dim=-1)
+                    new.append(nxt)
+        finally:
+            for s in seqs:
+                cache.close(s)
+        tokens = torch.stack(new, dim=1)
+        return [torch.cat((p.reshape(-1).to(device), t)) for p, t in zip(prompts, tokens)]
