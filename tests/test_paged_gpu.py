@@ -147,6 +147,22 @@ def test_flat_and_peaked_scores(cuda_ops, new, alpha):
     assert bool(((out.double().cpu() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("new,keys", [(1, 300), (150, 300), (150, 2000)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_from_zero(cuda_ops, new, keys, sign):
+    """All scores near +1800 or -1800 (in powers of two): only their differences count."""
+    dim = 64
+    b = make_batch([new], [keys], 1, 16, dim, 93)
+    b["k_pages"] = rand_s8(tuple(b["k_pages"].shape), 94, 90, 110)
+    q = torch.full((new, 2, dim), 100 * sign, dtype=torch.int8)
+    alpha = 2e-3
+    want, spread = P.paged_attention(q, *index_args(b), alpha, 0.02)
+    out = cuda_ops.paged_attention(q.cuda(), *index_args(cuda(b)), alpha_qk=alpha, alpha_pv=0.02, out_dtype=torch.float16)
+    s_max = alpha * 100 * 110 * dim * 1.4427
+    tol = spread * (2.0 ** -11 + 2.0 ** -15 + 2 * s_max * 2.0 ** -23) + want.abs() * 2.0 ** -11 * 1.001 + 2.0 ** -25
+    assert bool(((out.double().cpu() - want).abs() <= tol).all())
+
+
 def test_long_tail_of_small_weights(cuda_ops):
     """One key far above 4095 others (weights near 2^-20 each): the tail must not be rounded away."""
     dim, keys = 64, 4096

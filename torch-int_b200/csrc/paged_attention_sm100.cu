@@ -612,7 +612,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           const float old = off;
           if ((j == 0 || top > 15.f) && top > -INFINITY) off += top - 7.f;
           const float by = old - off;
-          const float corr = ex2(by);
+          const float corr = j > 0 ? ex2(by) : 1.f;    // in the first tile nothing is there to rescale, and 2^by may be infinite
           l *= corr;
           const float2 by2 = make_float2(by, by);
 #pragma unroll
