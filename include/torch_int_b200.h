@@ -32,6 +32,7 @@ extern "C" {
 #define TI_E_INVALID (-1) /* bad shape, alignment or pointer */
 #define TI_E_CUDA (-2)    /* a CUDA runtime / driver call failed */
 #define TI_E_DEVICE (-3)  /* returned by ti_check_device: a kernel's bounded wait gave up */
+#define TI_E_WORKSPACE (-4) /* ti_paged_attention: these sizes need a (larger) workspace; nothing was launched */
 
 /* ---- linear layers: out[M,N] = epilogue(input[M,K] . weight[N,K]^T, bias[N]) ---- */
 
@@ -310,7 +311,8 @@ int ti_paged_append(const ti_paged_batch* batch, const ti_paged_append_args* arg
  * ti_decode_attention_s8 the probabilities are not rounded to int8.  A token that sees no key (fewer keys than
  * new tokens) gives 0.  q int8, tokens ld_q elements apart; out_kind: 1 fp16, 2 bf16, 3 int8 (sat_rne).
  * max_kv_len bounds kv_lens.  `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
- * contents irrelevant, not shared by calls that may overlap on the GPU. */
+ * contents irrelevant, not shared by calls that may overlap on the GPU; NULL where that is 0 (a call that turns out
+ * to need one launches nothing and returns TI_E_WORKSPACE). */
 typedef struct ti_paged_attention_args {
   const int8_t* q;
   int64_t ld_q, q_heads, max_kv_len;

@@ -91,8 +91,8 @@ def test_bad_attention_arguments_are_refused(lib, base, change, words):
     a = dict(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1, alpha_qk=1.0, alpha_pv=1.0)
     a.update(change)
     args = PagedAttentionArgs(**a)
-    assert lib.ti_paged_attention(ctypes.byref(batch_of(base)), ctypes.byref(args), None) == -1
-    assert words in lib.ti_last_error()
+    rc = lib.ti_paged_attention(ctypes.byref(batch_of(base)), ctypes.byref(args), None)
+    assert rc == (-4 if words == b"workspace" else -1) and words in lib.ti_last_error()
 
 
 @pytest.mark.parametrize("change,words", [

@@ -192,7 +192,7 @@ __device__ __forceinline__ float2 ld_cluster8(uint32_t addr) {
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_rows_kernel(const PagedAttnParams p) {
+__device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   using SM = RowsSmem<D, NT>;
   constexpr int R = SM::R, LDO = SM::LDO;
   constexpr int MT = D / 16;  // 16-row tiles of O^T
@@ -205,8 +205,6 @@ __global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_r
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, a = lane & 3;
   const int b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles, h = blockIdx.y, split = blockIdx.x;
   PagedSeq s;
-  grid_dep_launch();
-  grid_dep_wait();
   if (!paged_sequence(v, b, p.max_kv_len, &s)) return;  // (returns before the keys are looked at: a whole cluster's)
   const int G = p.group, rows = s.T * G, r0 = rt * R;
   if (r0 >= rows || rows > p.rows_below) return;
@@ -456,6 +454,18 @@ __global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_r
   cluster_sync_all();  // the others may still read this CTA's part
 }
 
+// Launched as a programmatic dependent: of whatever comes before, which it waits for; or of the tile kernel of the
+// same call, beside which it runs on the SMs that kernel leaves free (their rows are different sequences').  Then only
+// its last CTA waits, at its end: the call is complete when this kernel is.
+template <int D, int NT>
+__global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_rows_kernel(const PagedAttnParams p) {
+  grid_dep_launch();
+  if (!p.beside_tiles) grid_dep_wait();
+  rows_of_a_cta<D, NT>(p);
+  if (p.beside_tiles && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+    grid_dep_wait();
+}
+
 // One block per (token, query head): joins the partial contexts of the row's splits, every fourth one in a warp (a
 // single warp took 14 us for 56 splits, most of it waiting for its loads), then the warps'.
 template <int D>
@@ -587,11 +597,22 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   if (pl.tiles) {
     pl.tile.tokens_per_tile = static_cast<int>(TILE_ROWS / group);
     pl.tile.pairs = static_cast<int>(div_up(max_query_len, 2 * pl.tile.tokens_per_tile));
-    const int64_t units = batch * kv_heads * pl.tile.pairs;
-    int64_t chunk = round_up(div_up(max_kv_len, units >= PAGED_SMS ? 1 : div_up(PAGED_SMS, units)), 128);
-    if (chunk < 512) chunk = 512;
-    pl.tile.chunk = static_cast<int>(chunk);
-    pl.tile.splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
+    // The keys are split where that makes the last round of CTAs shorter: rounds of (1.75 us per key tile + 4 us of fixed
+    // costs), as measured, against the partial results' way through memory (written and read at 5 TB/s, 3 us for the
+    // joining kernel).  128 units of 32 key tiles: 68 us whole, 111 split in two; 8 units of 128 tiles: 16 parts.
+    const int64_t units = batch * kv_heads * pl.tile.pairs, tiles = div_up(max_kv_len, 128);
+    double best = 0;
+    for (int64_t n = 1; n <= 64 && n <= (tiles > 0 ? tiles : 1); ++n) {
+      const int64_t part = div_up(tiles, n);
+      if (n > 1 && div_up(tiles, part) != n) continue;  // the same parts as a smaller n
+      const double us = static_cast<double>(div_up(units * n, PAGED_SMS)) * (1.75 * static_cast<double>(part) + 4.0) +
+                        (n > 1 ? 3.0 + static_cast<double>(tokens * group * kv_heads * n) * head_dim * 8 / 5e6 : 0.0);
+      if (n == 1 || us < best) {
+        best = us;
+        pl.tile.chunk = static_cast<int>(part > 0 ? part * 128 : 128);
+        pl.tile.splits = static_cast<int>(n);
+      }
+    }
     if (pl.tile.splits > pl.splits) pl.splits = pl.tile.splits;
   }
   return pl;
@@ -626,18 +647,12 @@ cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const Pla
 
 template <int D>
 int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaStream_t stream) {
-  if (pl.rows) {
-    const cudaError_t e = pl.nt == 1 ? launch_rows<D, 1>(b, p, pl, stream) : launch_rows<D, 2>(b, p, pl, stream);
-    if (e != cudaSuccess) {
-      set_error("paged_attention launch failed: %s", cudaGetErrorString(e));
-      return TI_E_CUDA;
-    }
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && pl.tiles) {
+  if (pl.tiles) {
     const int rc = launch_paged_tiles(b, p, pl.tile, stream);
     if (rc != TI_OK) return rc;
   }
+  cudaError_t e = cudaSuccess;
+  if (pl.rows) e = pl.nt == 1 ? launch_rows<D, 1>(b, p, pl, stream) : launch_rows<D, 2>(b, p, pl, stream);
   if (e == cudaSuccess && pl.splits > 1) {
     cudaLaunchConfig_t cfg = {};
     // only the rows of few-row sequences have partial results where the tile kernel does not split
@@ -707,10 +722,10 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   }
   const int64_t need = paged_attention_workspace_bytes(b.batch, b.tokens, a.q_heads, b.kv_heads, b.head_dim,
                                                        b.max_query_len, a.max_kv_len);
-  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 15) != 0)) {
+  if (need > a.workspace_bytes || (need > 0 && (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15) != 0))) {
     set_error("paged_attention: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
               (long long)a.workspace_bytes);
-    return TI_E_INVALID;
+    return TI_E_WORKSPACE;
   }
   int* status = status_word_ptr();
   if (!status) {
@@ -732,6 +747,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   p.chunk = pl.chunk;
   p.max_splits = pl.splits;
   p.cluster = pl.cluster;
+  p.beside_tiles = pl.tiles && pl.rows;
   p.rows_below = pl.tiles ? pl.few : 0x7FFFFFFF;
   if (!pl.rows) p.rows_below = 0;
   p.part_o = static_cast<float*>(a.workspace);

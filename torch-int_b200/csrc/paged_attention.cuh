@@ -26,6 +26,7 @@ struct PagedAttnParams {
   int max_splits;     // stride of the partial results
   int cluster;        // the splits of the rows kernel are a cluster and need no partial results
   int rows_below;     // sequences with at most this many rows belong to the rows kernel, the others to the tile kernel
+  int beside_tiles;   // the rows kernel follows the tile kernel of the same call without waiting for it
   float* part_o;      // [tokens * q_heads][max_splits][head_dim], unnormalised
   float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
 };

@@ -633,37 +633,36 @@ _PAGED_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.in
 def _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, tokens, max_query_len):
     """Checks the cache and the index tensors of a ragged batch; returns the packed ti_paged_batch, the device index
     and the sizes (sequences, heads, page_size, head_dim, block table width, bound of the new tokens)."""
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"),
-                    (query_starts, "query_starts"), (kv_lens, "kv_lens")):
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"{name} must be a torch.Tensor")
-    shape = k_pages.shape
-    dev = k_pages.get_device()
-    if not (dev >= 0 and len(shape) == 4 and k_pages.dtype is torch.int8 and v_pages.dtype is torch.int8
-            and v_pages.shape == shape and v_pages.get_device() == dev
-            and k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise RuntimeError("k_pages and v_pages must be contiguous CUDA int8 tensors of the same shape "
-                           "[pages, kv_heads, page_size, head_dim]")
-    if not (block_table.dtype is torch.int32 and query_starts.dtype is torch.int32 and kv_lens.dtype is torch.int32
-            and block_table.get_device() == dev and query_starts.get_device() == dev and kv_lens.get_device() == dev):
-        raise RuntimeError("block_table, query_starts and kv_lens must be int32 tensors on the cache's device")
-    table = block_table.shape
-    batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if len(table) != 2 or table[0] != batch or query_starts.shape != (batch + 1,):
-        raise RuntimeError(f"block_table {tuple(table)}, query_starts {tuple(query_starts.shape)} and kv_lens "
-                           f"{tuple(kv_lens.shape)} must be [B, pages], [B + 1] and [B]")
-    width = table[1]
-    stride, inner = block_table.stride()
-    if batch <= 1:
-        stride = width
-    if (width > 1 and inner != 1) or stride < width or not (query_starts.is_contiguous() and kv_lens.is_contiguous()):
-        raise RuntimeError("block_table rows, query_starts and kv_lens must be packed")
-    if max_query_len is None or max_query_len > tokens:
-        max_query_len = tokens
-    pages, hkv, page_size, d = shape
-    packed = _pack_paged_batch(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(),
-                               kv_lens.data_ptr(), pages, hkv, page_size, d, stride, width, batch, tokens, max_query_len)
-    return packed, dev, batch, hkv, page_size, d, width, max_query_len
+    try:
+        shape = k_pages.shape
+        dev = k_pages.get_device()
+        if not (dev >= 0 and len(shape) == 4 and k_pages.dtype is torch.int8 and v_pages.dtype is torch.int8
+                and v_pages.shape == shape and v_pages.get_device() == dev
+                and k_pages.is_contiguous() and v_pages.is_contiguous()):
+            raise RuntimeError("k_pages and v_pages must be contiguous CUDA int8 tensors of the same shape "
+                               "[pages, kv_heads, page_size, head_dim]")
+        if not (block_table.dtype is query_starts.dtype is kv_lens.dtype is torch.int32
+                and block_table.get_device() == query_starts.get_device() == kv_lens.get_device() == dev):
+            raise RuntimeError("block_table, query_starts and kv_lens must be int32 tensors on the cache's device")
+        table = block_table.shape
+        batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+        if len(table) != 2 or table[0] != batch or query_starts.shape != (batch + 1,):
+            raise RuntimeError(f"block_table {tuple(table)}, query_starts {tuple(query_starts.shape)} and kv_lens "
+                               f"{tuple(kv_lens.shape)} must be [B, pages], [B + 1] and [B]")
+        width = table[1]
+        stride, inner = block_table.stride()
+        if batch <= 1:
+            stride = width
+        if (width > 1 and inner != 1) or stride < width or not (query_starts.is_contiguous() and kv_lens.is_contiguous()):
+            raise RuntimeError("block_table rows, query_starts and kv_lens must be packed")
+        if max_query_len is None or max_query_len > tokens:
+            max_query_len = tokens
+        pages, hkv, page_size, d = shape
+        return (_pack_paged_batch(k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), query_starts.data_ptr(),
+                                  kv_lens.data_ptr(), pages, hkv, page_size, d, stride, width, batch, tokens,
+                                  max_query_len), dev, batch, hkv, page_size, d, width, max_query_len)
+    except AttributeError:
+        raise RuntimeError("k_pages, v_pages, block_table, query_starts and kv_lens must be tensors") from None
 
 
 def _paged_rows(t, name, tokens, d, dev, dtype):
@@ -678,17 +677,18 @@ def _paged_rows(t, name, tokens, d, dev, dtype):
     return h, token if n > 1 else h * d
 
 
+_E_WORKSPACE = -4
+
+
 def _paged_call(fn, batch, args, dev):
     cur = _current_device()
     if cur == dev:
-        rc = fn(batch, args, _raw_stream(dev))
-    else:
-        torch.cuda.set_device(dev)
-        try:
-            rc = fn(batch, args, _raw_stream(dev))
-        finally:
-            torch.cuda.set_device(cur)
-    _check(rc)
+        return fn(batch, args, _raw_stream(dev))
+    torch.cuda.set_device(dev)
+    try:
+        return fn(batch, args, _raw_stream(dev))
+    finally:
+        torch.cuda.set_device(cur)
 
 
 def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, max_query_len=None, q=None,
@@ -714,7 +714,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     out = None
     if q is not None:
         hq, ld_q = _paged_rows(q, "q", n, d, dev, dtype)
-        out = q.new_empty((n, hq, d), dtype=torch.int8)
+        out = torch.empty_like(q, dtype=torch.int8)  # packed, whatever the stride of q's tokens
         q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
     if rotary is not None:
         if not (isinstance(rotary, torch.Tensor) and rotary.dtype is torch.float32 and rotary.get_device() == dev
@@ -724,7 +724,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
         rot_ptr = rotary.data_ptr()
     args = _pack_paged_append(q_ptr, k.data_ptr(), v.data_ptr(), ld_q, ld_k, ld_v, hq, rot_ptr, rows, rd, out_ptr,
                               q_alpha, k_alpha, v_alpha, _PAGED_DTYPES[dtype], 1 if interleaved else 0)
-    _paged_call(_c_paged_append, batch, args, dev)
+    _check(_paged_call(_c_paged_append, batch, args, dev))
     return out
 
 
@@ -747,18 +747,20 @@ def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     if max_kv_len is None:
         max_kv_len = width * page_size
     if out is None:
-        out = q.new_empty((n, hq, d), dtype=out_dtype)
+        out = torch.empty_like(q, dtype=out_dtype)  # packed, whatever the stride of q's tokens
     elif not (isinstance(out, torch.Tensor) and out.get_device() == dev and out.shape == q.shape and out.is_contiguous()):
         raise RuntimeError(f"out must be a contiguous {tuple(q.shape)} tensor on the cache's device")
     kind = _PAGED_DTYPES.get(out.dtype, 0)
     if kind == 0:
         raise RuntimeError(f"the context must be int8, float16 or bfloat16, not {out.dtype}")
-    need = _c_paged_workspace(b, n, hq, hkv, d, max_q, max_kv_len)
-    # scratch of this call alone: the allocator orders its reuse by stream, and a captured graph keeps its own
-    ws = q.new_empty(need) if need else None
-    args = _pack_paged_attention(q.data_ptr(), ld_q, hq, max_kv_len, out.data_ptr(), ws.data_ptr() if need else 0,
-                                 need, alpha_qk, alpha_pv, kind)
-    _paged_call(_c_paged_attention, batch, args, dev)
+    args = (q.data_ptr(), ld_q, hq, max_kv_len, out.data_ptr())
+    rc = _paged_call(_c_paged_attention, batch, _pack_paged_attention(*args, 0, 0, alpha_qk, alpha_pv, kind), dev)
+    if rc == _E_WORKSPACE:
+        # scratch of this call alone: the allocator orders its reuse by stream, and a captured graph keeps its own
+        need = _c_paged_workspace(b, n, hq, hkv, d, max_q, max_kv_len)
+        ws = q.new_empty(need)
+        rc = _paged_call(_c_paged_attention, batch, _pack_paged_attention(*args, ws.data_ptr(), need, alpha_qk, alpha_pv, kind), dev)
+    _check(rc)
     return out
 
 
