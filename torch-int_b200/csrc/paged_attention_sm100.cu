@@ -134,6 +134,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
   return *reinterpret_cast<const float2*>(&d);
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -659,67 +666,87 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         tc_fence_before();
         mbar_arrive(smem_u32(&p_full[x]));
       }
-      if (tiles > 0) {
-        wait(&o_full[x], o_phase, TI_ERR_PT_O_FULL);
-        o_phase ^= 1;
-        tc_fence_after();
-      }
+      // What the epilogue needs, while the last product runs.  The item is read again and `row` is opaque, so that
+      // nothing of this is carried through the loop above.
       s_sum[(x * 2 + half) * TILE + r] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l = s_sum[x * 2 * TILE + r] + s_sum[(x * 2 + 1) * TILE + r];
-      // The item is read again and `row` is opaque, so that nothing of this is carried through the loop above.
       int row = r;
       asm volatile("" : "+r"(row));
       const int split = item[rq.stage].split, n_splits = item[rq.stage].n_splits;
       const int t = item[rq.stage].t0 + x * TPT + r_token;
       // beyond the keys of this pair of row tiles there is nothing to write
-      const bool valid = ok && row < G * TPT && t < item[rq.stage].T && split < n_splits;
+      const bool valid = row < G * TPT && t < item[rq.stage].T && split < n_splits;
       const bool whole = n_splits == 1;
       long long at = static_cast<long long>(item[rq.stage].q0 + t) * p.q_heads + item[rq.stage].h * G + (row - r_token * G);
       if (!whole) at = at * p.max_splits + split;
       const float scale = !whole ? 1.f : l > 0.f ? p.alpha_pv / l : 0.f;
-      if (valid && !whole && half == 0) p.part_ml[at] = make_float2(l > 0.f ? off : -1e30f, l);
+      if (ok && valid && !whole && half == 0) p.part_ml[at] = make_float2(l > 0.f ? off : -1e30f, l);
       // Context rows.  A thread holds a row; stored from there, a warp would touch 32 rows with every instruction.  So
       // 64 bytes of each row at a time pass through shared memory - the item's query tile, which nobody reads any more -
-      // and every group of four lanes stores one row's.  Loops of few instructions: this code is cold each time it is
+      // and every group of four lanes stores one row's.  A loop of few instructions: this code is cold each time it is
       // reached, and fetching it unrolled took longer (4200 clocks) than the stores.
       const int width = !whole ? 4 : p.out_kind == 3 ? 1 : 2;  // bytes of an element
-      uint8_t* out = whole ? static_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o);
-      const long long row_bytes = (at * D + col0) * width;
-      uint8_t* stage = smem + SM::Q + (rq.stage * 2 + x) * TILE_BYTES + (half * 4 + (warp & 3)) * 2048;
-#pragma unroll 1
-      for (int col = 0; col < cols; col += 8) {
-        uint32_t o[8];
-        tmem_ld_32x8(to + col, o);
-        tmem_ld_wait();
-        float y[8];
+      const int c16 = (lane & 3) * 16, swz = (lane >> 1) & 3, swz_out = (lane >> 3) & 3;
+      const long long row_bytes = valid ? (at * D + col0) * width : -1;
+      uint8_t* dst[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = tiles > 0 ? __uint_as_float(o[i]) * scale : 0.f;
-        const int byte = (col * width) & 63;
-        const int piece = byte >> 4, swz = (lane >> 1) & 3;
-        uint8_t* dst = stage + lane * 64;
-        if (width == 4) {
-          *reinterpret_cast<float4*>(dst + ((piece ^ swz) << 4)) = make_float4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<float4*>(dst + (((piece + 1) ^ swz) << 4)) = make_float4(y[4], y[5], y[6], y[7]);
-        } else if (width == 2) {
-          *reinterpret_cast<uint4*>(dst + ((piece ^ swz) << 4)) =
-              make_uint4(paged_pack2(p.out_kind, y[0], y[1]), paged_pack2(p.out_kind, y[2], y[3]),
-                         paged_pack2(p.out_kind, y[4], y[5]), paged_pack2(p.out_kind, y[6], y[7]));
-        } else {
-          *reinterpret_cast<uint2*>(dst + ((piece ^ swz) << 4) + (byte & 8)) =
-              make_uint2(paged_pack4_s8(y[0], y[1], y[2], y[3]), paged_pack4_s8(y[4], y[5], y[6], y[7]));
-        }
-        if (byte + 8 * width == 64 || col + 8 == cols) {
-          __syncwarp();
-          const int done = col * width - byte, c16 = (lane & 3) * 16;
+      for (int i = 0; i < 4; ++i) {
+        const long long to_row = __shfl_sync(0xffffffffu, row_bytes, 8 * i + (lane >> 2));
+        dst[i] = to_row < 0 ? nullptr : (whole ? static_cast<uint8_t*>(p.out) : reinterpret_cast<uint8_t*>(p.part_o)) + to_row + c16;
+      }
+      uint8_t* stage = smem + SM::Q + (rq.stage * 2 + x) * TILE_BYTES + (half * 4 + (warp & 3)) * 2048;
+      if (tiles > 0) {
+        wait(&o_full[x], o_phase, TI_ERR_PT_O_FULL);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
 #pragma unroll 1
-          for (int i = 0; i < 32; i += 8) {
-            const int rr = i + (lane >> 2);
-            const long long base = __shfl_sync(0xffffffffu, row_bytes, rr);
-            const bool there = __shfl_sync(0xffffffffu, static_cast<int>(valid), rr) != 0;
-            if (there && c16 < byte + 8 * width)
-              *reinterpret_cast<uint4*>(out + base + done + c16) =
-                  *reinterpret_cast<const uint4*>(stage + rr * 64 + (c16 ^ (((rr >> 1) & 3) << 4)));
+      for (int col = 0; col < cols; col += 16) {
+        uint32_t o[16];
+        tmem_ld_32x16(to + col, o);
+        tmem_ld_wait();
+        if (tiles == 0) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float2 y = mul2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(scale, scale));
+          o[i] = __float_as_uint(y.x);
+          o[i + 1] = __float_as_uint(y.y);
+        }
+        const int byte = (col * width) & 63, filled = byte + 16 * width;
+        uint8_t* mine = stage + lane * 64;
+        auto put = [&](int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+          *reinterpret_cast<uint4*>(mine + ((((byte >> 4) + piece) ^ swz) << 4)) = make_uint4(a, b, c, d);
+        };
+        auto y = [&](int i) { return __uint_as_float(o[i]); };
+        if (width == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) put(i, o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if (width == 2) {
+          uint32_t h[8];
+          if (p.out_kind == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = paged_pack2(2, y(2 * i), y(2 * i + 1));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = paged_pack2(1, y(2 * i), y(2 * i + 1));
+          }
+          put(0, h[0], h[1], h[2], h[3]);
+          put(1, h[4], h[5], h[6], h[7]);
+        } else {
+          put(0, paged_pack4_s8(y(0), y(1), y(2), y(3)), paged_pack4_s8(y(4), y(5), y(6), y(7)),
+              paged_pack4_s8(y(8), y(9), y(10), y(11)), paged_pack4_s8(y(12), y(13), y(14), y(15)));
+        }
+        if (filled == 64 || col + 16 == cols) {
+          __syncwarp();
+          const uint8_t* src = stage + (lane >> 2) * 64 + (c16 ^ (swz_out << 4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (ok && dst[i] && c16 < filled) *reinterpret_cast<uint4*>(dst[i]) = *reinterpret_cast<const uint4*>(src + 512 * i);
+            if (dst[i]) dst[i] += 64;
           }
           __syncwarp();
         }
