@@ -39,8 +39,6 @@
 namespace ti {
 namespace {
 
-constexpr int ROWS_WARPS = 4;
-constexpr int ROWS_THREADS = ROWS_WARPS * 32;
 constexpr int STAGES = 2;           // steps of a warp in shared memory: one in flight, one in use
 constexpr int STEP = 32;            // keys of a step: two groups of 16
 constexpr int MAX_CLUSTER = 8;
@@ -166,17 +164,17 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// CTAs of paged_rows_kernel an SM holds: registers (147 per thread of 128-wide heads) and the queues' 64 KB.
-__host__ __device__ constexpr int rows_ctas_per_sm(int head_dim, int nt) {
-  return head_dim == 128 ? (nt == 1 ? 3 : 2) : (nt == 1 ? 4 : 3);
+// CTAs of paged_rows_kernel an SM holds: registers (147 per thread of 128-wide heads) and the queues' 16 KB a warp.
+__host__ __device__ constexpr int rows_ctas_per_sm(int head_dim, int nt, int warps) {
+  return (head_dim == 128 ? (nt == 1 ? 12 : 8) : (nt == 1 ? 16 : 12)) / warps;
 }
 
 // Shared memory of a rows CTA: the warps' queues; when they are empty, the warps' contexts and what they join to.
-template <int D, int NT>
+template <int D, int NT, int WARPS>
 struct RowsSmem {
   static constexpr int R = 8 * NT, LDO = D + 4;
-  static constexpr int STAGE = 2 * Group<D>::BYTES, QUEUE = ROWS_WARPS * STAGES * STAGE;
-  static constexpr int JOINED = ROWS_WARPS * R * LDO * 4;          // fp32 [R][D]
+  static constexpr int STAGE = 2 * Group<D>::BYTES, QUEUE = WARPS * STAGES * STAGE;
+  static constexpr int JOINED = WARPS * R * LDO * 4;          // fp32 [R][D]
   static constexpr int BYTES = QUEUE > JOINED + R * D * 4 ? QUEUE : JOINED + R * D * 4;
 };
 
@@ -191,19 +189,22 @@ __device__ __forceinline__ float2 ld_cluster8(uint32_t addr) {
   return x;
 }
 
-template <int D, int NT>
+template <int D, int NT, int WARPS>
 __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
-  using SM = RowsSmem<D, NT>;
+  using SM = RowsSmem<D, NT, WARPS>;
   constexpr int R = SM::R, LDO = SM::LDO;
   constexpr int MT = D / 16;  // 16-row tiles of O^T
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_m[ROWS_WARPS][R], s_l[ROWS_WARPS][R];
+  __shared__ float s_m[WARPS][R], s_l[WARPS][R];
   __shared__ float2 s_ml[R];
   float(*s_o)[R][LDO] = reinterpret_cast<float(*)[R][LDO]>(smem);
   float* s_join = reinterpret_cast<float*>(smem + SM::JOINED);
   const PagedView& v = p.view;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, a = lane & 3;
   const int b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles, h = blockIdx.y, split = blockIdx.x;
+  // the first entries of the block table are loaded beside the lengths, not behind them (one latency less)
+  const unsigned first_page = static_cast<unsigned>(split * p.chunk + (warp + WARPS * (lane >> 1)) * STEP + (lane & 1) * 16) >> v.page_shift;
+  const int first_entry = first_page < static_cast<unsigned>(v.table_width) ? v.table[b * v.table_ld + first_page] : -1;
   PagedSeq s;
   if (!paged_sequence(v, b, p.max_kv_len, &s)) return;  // (returns before the keys are looked at: a whole cluster's)
   const int G = p.group, rows = s.T * G, r0 = rt * R;
@@ -213,20 +214,21 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   if (split >= sp.n && (!p.cluster || sp.n == 1)) return;
   const int k0 = min(split * p.chunk, sp.keys), k1 = min(k0 + p.chunk, sp.keys);
 
-  // this warp's steps: keys k0 + (warp + ROWS_WARPS * i) * STEP, i < cnt; lane n knows the page of group n of 32
+  // this warp's steps: keys k0 + (warp + WARPS * i) * STEP, i < cnt; lane n knows the page of group n of 32
   const int steps = (k1 - k0 + STEP - 1) / STEP;
-  const int cnt = steps > warp ? (steps - warp + ROWS_WARPS - 1) / ROWS_WARPS : 0;
+  const int cnt = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;
   const uint32_t queue = smem_u32(smem) + warp * STAGES * SM::STAGE;
   int my_page = 0;
   auto fetch = [&](int i) {  // in order, every i < cnt once
     if (i < cnt) {
       if ((i & 15) == 0) {
-        const int key = k0 + (warp + ROWS_WARPS * (i + (lane >> 1))) * STEP + (lane & 1) * 16;
-        my_page = key < k1 ? max(0, paged_page(v, b, key >> v.page_shift)) : 0;
+        const int key = k0 + (warp + WARPS * (i + (lane >> 1))) * STEP + (lane & 1) * 16;
+        my_page = 0;
+        if (key < k1) my_page = max(0, i == 0 ? paged_checked(v, first_entry) : paged_page(v, b, key >> v.page_shift));
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int key = k0 + (warp + ROWS_WARPS * i) * STEP + n * 16;
+        const int key = k0 + (warp + WARPS * i) * STEP + n * 16;
         const long long page = __shfl_sync(0xffffffffu, my_page, (i & 15) * 2 + n);
         const long long at = (((page * v.kv_heads + h) << v.page_shift) + (key & ((1 << v.page_shift) - 1))) * D;
         if (key < k1)
@@ -264,7 +266,7 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   }
 #pragma unroll 1
   for (int i = 0; i < cnt; ++i) {
-    const int key = k0 + (warp + ROWS_WARPS * i) * STEP;
+    const int key = k0 + (warp + WARPS * i) * STEP;
     const uint8_t* stage = smem + (warp * STAGES + i % STAGES) * SM::STAGE;
     copy_wait<STAGES - 2>();
     __syncwarp();  // step i has landed, and every lane is done with the one whose place the next fetch takes
@@ -393,15 +395,15 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   }
   __syncthreads();
   const int work = min(R, rows - r0) * (D / 4);
-  for (int i = threadIdx.x; i < work; i += ROWS_THREADS) {
+  for (int i = threadIdx.x; i < work; i += WARPS * 32) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
     float mx = s_m[0][r];
 #pragma unroll
-    for (int w = 1; w < ROWS_WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
+    for (int w = 1; w < WARPS; ++w) mx = fmaxf(mx, s_m[w][r]);
     float sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < ROWS_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float f = exp2f(s_m[w][r] - mx);
       const float4 y = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
       sum += f * s_l[w][r];
@@ -425,7 +427,7 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   // ---- join the splits of the cluster (rank = split), each CTA a part of the rows and columns
   cluster_sync_all();
   const uint32_t join_at = smem_u32(s_join), ml_at = smem_u32(s_ml);
-  for (int i = split * ROWS_THREADS + threadIdx.x; i < work; i += static_cast<int>(gridDim.x) * ROWS_THREADS) {
+  for (int i = split * WARPS * 32 + threadIdx.x; i < work; i += static_cast<int>(gridDim.x) * WARPS * 32) {
     const int r = i / (D / 4), d = (i % (D / 4)) * 4, row = r0 + r;
     float mx = -1e30f, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -457,11 +459,11 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
 // Launched as a programmatic dependent: of whatever comes before, which it waits for; or of the tile kernel of the
 // same call, beside which it runs on the SMs that kernel leaves free (their rows are different sequences').  Then only
 // its last CTA waits, at its end: the call is complete when this kernel is.
-template <int D, int NT>
-__global__ void __launch_bounds__(ROWS_THREADS, rows_ctas_per_sm(D, NT)) paged_rows_kernel(const PagedAttnParams p) {
+template <int D, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, rows_ctas_per_sm(D, NT, WARPS)) paged_rows_kernel(const PagedAttnParams p) {
   grid_dep_launch();
   if (!p.beside_tiles) grid_dep_wait();
-  rows_of_a_cta<D, NT>(p);
+  rows_of_a_cta<D, NT, WARPS>(p);
   if (p.beside_tiles && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
     grid_dep_wait();
 }
@@ -558,7 +560,8 @@ constexpr int MIN_CHUNK = 512, MAX_CHUNK = 2048;  // keys of a split of paged_ro
 struct Plan {
   bool rows, tiles;
   int few;
-  int nt, row_tiles, chunk, row_splits;  // rows kernel: 8-row tiles of a CTA, CTAs of a sequence, keys of a split
+  int nt, warps;                         // rows kernel: 8-row tiles and warps of a CTA
+  int row_tiles, chunk, row_splits;      // CTAs of a sequence, keys of a split
   bool cluster;                          // the splits of the rows kernel are a cluster
   PagedTilePlan tile;
   int splits;                            // most splits that go through the workspace: stride of the partial results
@@ -585,11 +588,15 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     // 64 contexts of up to 8192 keys took 94 us in pieces of 1024 to 2048 keys, 102 in whole).  Otherwise as many pieces
     // as fill the SMs once (two contexts of 131072 keys: 82 us so, 110 with a third more pieces), of at least MIN_CHUNK
     // keys (one context of 500 keys: 7.6 us in one piece, 8.8 in four).
-    const int64_t units = batch * kv_heads * pl.row_tiles, slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt);
+    const int64_t units = batch * kv_heads * pl.row_tiles, slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 4);
     int64_t chunk = units >= slots ? MAX_CHUNK : round_up(div_up(max_kv_len, slots / units), STEP);
     if (chunk < MIN_CHUNK) chunk = MIN_CHUNK;
     pl.chunk = static_cast<int>(chunk);
     pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
+    // Three warps to a CTA instead of four where the work then runs in fewer rounds, by more than each takes longer:
+    // 8 sequences of 512 keys, 56 heads (448 units; 444 CTAs of four warps at a time, 592 of three): 21.0 -> 17.8 us.
+    const int64_t slots3 = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 3);
+    pl.warps = pl.nt == 1 && pl.row_splits == 1 && 4 * div_up(units, slots3) < 3 * div_up(units, slots) ? 3 : 4;
     // a cluster holds its CTAs until the last one is done: only where all of them run at once
     pl.cluster = pl.row_splits > 1 && pl.row_splits <= MAX_CLUSTER && units * pl.row_splits <= slots;
     if (!pl.cluster) pl.splits = pl.row_splits;
@@ -618,10 +625,10 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   return pl;
 }
 
-template <int D, int NT>
+template <int D, int NT, int WARPS>
 cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaStream_t stream) {
-  auto kernel = paged_rows_kernel<D, NT>;
-  constexpr int smem = RowsSmem<D, NT>::BYTES;
+  auto kernel = paged_rows_kernel<D, NT, WARPS>;
+  constexpr int smem = RowsSmem<D, NT, WARPS>::BYTES;
   static PagedOncePerDevice once;
   const cudaError_t e = once.run([kernel] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -630,7 +637,7 @@ cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const Pla
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
                      static_cast<unsigned>(b.batch * pl.row_tiles));
-  cfg.blockDim = dim3(ROWS_THREADS);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -652,7 +659,10 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
     if (rc != TI_OK) return rc;
   }
   cudaError_t e = cudaSuccess;
-  if (pl.rows) e = pl.nt == 1 ? launch_rows<D, 1>(b, p, pl, stream) : launch_rows<D, 2>(b, p, pl, stream);
+  if (pl.rows)
+    e = pl.warps == 3 ? launch_rows<D, 1, 3>(b, p, pl, stream)
+        : pl.nt == 1  ? launch_rows<D, 1, 4>(b, p, pl, stream)
+                      : launch_rows<D, 2, 4>(b, p, pl, stream);
   if (e == cudaSuccess && pl.splits > 1) {
     cudaLaunchConfig_t cfg = {};
     // only the rows of few-row sequences have partial results where the tile kernel does not split

@@ -59,14 +59,17 @@ __device__ __forceinline__ bool paged_sequence(const PagedView& v, int b, int ma
   return ok;
 }
 
-// Page of block table entry `i` of sequence b.  An entry outside the pool sets status 212 and gives -1.
-__device__ __forceinline__ int paged_page(const PagedView& v, int b, int i) {
-  const int page = v.table[b * v.table_ld + i];
+// A block table entry that is in use.  One outside the pool sets status 212 and gives -1.
+__device__ __forceinline__ int paged_checked(const PagedView& v, int page) {
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(v.num_pages)) {
     atomicCAS(v.status, 0, static_cast<int>(TI_ERR_PAGED_PAGE));
     return -1;
   }
   return page;
+}
+// Page of block table entry `i` of sequence b.
+__device__ __forceinline__ int paged_page(const PagedView& v, int b, int i) {
+  return paged_checked(v, v.table[b * v.table_ld + i]);
 }
 
 }  // namespace ti
