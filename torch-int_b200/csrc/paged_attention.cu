@@ -468,21 +468,35 @@ __global__ void __launch_bounds__(WARPS * 32, rows_ctas_per_sm(D, NT, WARPS)) pa
     grid_dep_wait();
 }
 
-// One block per (token, query head): joins the partial contexts of the row's splits, every fourth one in a warp (a
-// single warp took 14 us for 56 splits, most of it waiting for its loads), then the warps'.
-template <int D>
+// Joins the partial contexts of the splits of a row = (token, query head).  A block has 4 / W rows; W = 4 warps share a
+// row's splits where there are many (a single warp took 14 us for 56 splits, most of it waiting for its loads), W = 1
+// has one warp for each row (16384 rows of two splits: 39 us -> 12).  blockIdx.y is the sequence and the row one of
+// it, or - by_token - the row is one of the call and the warp looks its sequence up.
+template <int D, int W>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParams p, int few_rows, int many_rows,
-                                                            int many_chunk) {
+                                                            int many_chunk, bool by_token) {
   __shared__ float4 s_x[4][32];
   __shared__ float s_m[4], s_l[4];
   const PagedView& v = p.view;
-  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x;  // (token, head) of the sequence
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = W == 1 ? 0 : warp;
+  const unsigned row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x;
+  const int head = row % p.q_heads;
+  int t = row / p.q_heads, b = blockIdx.y;
+  // (The index arrays are read before the wait: no kernel that lets its dependents start early writes them.)
+  if (by_token) {
+    b = -1;
+    for (int i = lane; i < v.batch; i += 32) {
+      const int q0 = v.query_starts[i], q1 = v.query_starts[i + 1];
+      if (q0 >= 0 && q0 <= t && t < q1 && q1 <= v.tokens && q1 - q0 <= v.max_query_len) b = i;
+    }
+    b = __reduce_max_sync(0xffffffffu, b);
+  }
   PagedSeq s;
-  const bool ok = paged_sequence(v, b, p.max_kv_len, &s);
+  const bool ok = b >= 0 && paged_sequence(v, b, p.max_kv_len, &s);
   grid_dep_wait();
-  const int t = row / p.q_heads, head = row % p.q_heads;
-  if (!ok || t >= s.T) return;
+  if (!ok) return;
+  if (by_token) t -= s.q0;
+  if (t >= s.T) return;
   // the row tile this row belonged to decides how many keys, hence splits, were visited
   const int G = p.group, rows = s.T * G;
   const bool many = rows > p.rows_below;
@@ -498,16 +512,20 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
   float mx = -1e30f, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int BATCH = 8;  // splits whose loads are in flight together
-  for (int i0 = warp; i0 < sp.n; i0 += 4 * BATCH) {
+  for (int i0 = part; i0 < sp.n; i0 += W * BATCH) {
     float2 e[BATCH];
     float4 y[BATCH];
     float top = mx;
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const int i = min(i0 + 4 * k, sp.n - 1);
-      e[k] = ml[i];
-      y[k] = *reinterpret_cast<const float4*>(po + static_cast<long long>(i) * D);
-      if (i0 + 4 * k >= sp.n) e[k] = make_float2(-1e30f, 0.f);
+      const int i = min(i0 + W * k, sp.n - 1);
+      const bool there = i0 + W * k < sp.n;
+      y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (W > 1 || there) {  // (with many splits a load too many costs less than a branch)
+        e[k] = ml[i];
+        y[k] = *reinterpret_cast<const float4*>(po + static_cast<long long>(i) * D);
+      }
+      if (!there) e[k] = make_float2(-1e30f, 0.f);
     }
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) top = fmaxf(top, e[k].x);
@@ -520,7 +538,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
     x.w *= corr;
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
-      const float f = i0 + 4 * k < sp.n ? exp2f(e[k].x - mx) : 0.f;
+      const float f = i0 + W * k < sp.n ? exp2f(e[k].x - mx) : 0.f;
       sum += f * e[k].y;
       x.x += f * y[k].x;
       x.y += f * y[k].y;
@@ -528,27 +546,29 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
       x.w += f * y[k].w;
     }
   }
-  s_x[warp][lane] = x;
-  if (lane == 0) {
-    s_m[warp] = mx;
-    s_l[warp] = sum;
-  }
-  __syncthreads();
-  if (warp != 0 || !mine) return;
-  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  sum = 0.f;
-  x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if constexpr (W > 1) {
+    s_x[warp][lane] = x;
+    if (lane == 0) {
+      s_m[warp] = mx;
+      s_l[warp] = sum;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    sum = 0.f;
+    x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = exp2f(s_m[w] - mx);
-    const float4 y = s_x[w][lane];
-    sum += f * s_l[w];
-    x.x += f * y.x;
-    x.y += f * y.y;
-    x.z += f * y.z;
-    x.w += f * y.w;
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(s_m[w] - mx);
+      const float4 y = s_x[w][lane];
+      sum += f * s_l[w];
+      x.x += f * y.x;
+      x.y += f * y.y;
+      x.z += f * y.z;
+      x.w += f * y.w;
+    }
   }
-  paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
+  if (mine) paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
 }
 
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
@@ -604,16 +624,26 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   if (pl.tiles) {
     pl.tile.tokens_per_tile = static_cast<int>(TILE_ROWS / group);
     pl.tile.pairs = static_cast<int>(div_up(max_query_len, 2 * pl.tile.tokens_per_tile));
-    // The keys are split where that makes the last round of CTAs shorter: rounds of (1.75 us per key tile + 4 us of fixed
-    // costs), as measured, against the partial results' way through memory (written and read at 5 TB/s, 3 us for the
-    // joining kernel).  128 units of 32 key tiles: 68 us whole, 111 split in two; 8 units of 128 tiles: 16 parts.
-    const int64_t units = batch * kv_heads * pl.tile.pairs, tiles = div_up(max_kv_len, 128);
+    // The keys are split where that makes the last round of CTAs shorter: rounds of (1.8 us per key tile + 4 us of fixed
+    // costs), as measured, against the partial results' way through memory (written and read at 5 TB/s, 6 us for the
+    // joining kernel).  One prompt of 512 tokens behind 3488, 32 query heads: 64 items of 32 key tiles on 148 SMs take 65 us
+    // whole, 48 in two parts, 52 in four; 16 items (8 query heads) 65 whole, 28 in four parts, 21.5 in nine; a chunk of 2048
+    // behind 14336 tokens (256 items) 449 whole, 500 and 458.  Sequences with few rows run on the SMs left free, so their
+    // share (at their bounds and 6.5 TB/s) counts as occupied SMs: the 512 tokens with 15 decoding sequences
+    // beside them take 74 us whole and 80 in two parts.
+    // The items are estimated from the number of tokens: of a batch that mixes a prompt with decoding sequences, the
+    // bounds alone would count every sequence as a prompt.
+    const int64_t by_tokens = div_up(tokens, 2 * pl.tile.tokens_per_tile), by_bounds = batch * pl.tile.pairs;
+    const int64_t units = kv_heads * (by_tokens < by_bounds ? by_tokens : by_bounds), tiles = div_up(max_kv_len, 128);
+    const double beside = pl.rows ? static_cast<double>((batch - 1) * max_kv_len * kv_heads) * head_dim * 2 / 6.5e6 : 0.0;
     double best = 0;
     for (int64_t n = 1; n <= 64 && n <= (tiles > 0 ? tiles : 1); ++n) {
       const int64_t part = div_up(tiles, n);
       if (n > 1 && div_up(tiles, part) != n) continue;  // the same parts as a smaller n
-      const double us = static_cast<double>(div_up(units * n, PAGED_SMS)) * (1.75 * static_cast<double>(part) + 4.0) +
-                        (n > 1 ? 3.0 + static_cast<double>(tokens * group * kv_heads * n) * head_dim * 8 / 5e6 : 0.0);
+      const double item = 1.8 * static_cast<double>(part) + 4.0, alone = static_cast<double>(div_up(units * n, PAGED_SMS)) * item;
+      const double shared = static_cast<double>(units * n) * item / PAGED_SMS + beside;
+      const double us = (alone > shared ? alone : shared) +
+                        (n > 1 ? 6.0 + static_cast<double>(tokens * group * kv_heads * n) * head_dim * 8 / 5e6 : 0.0);
       if (n == 1 || us < best) {
         best = us;
         pl.tile.chunk = static_cast<int>(part > 0 ? part * 128 : 128);
@@ -667,8 +697,13 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
     cudaLaunchConfig_t cfg = {};
     // only the rows of few-row sequences have partial results where the tile kernel does not split
     const int64_t few_tokens = pl.few / p.group;
-    const int64_t tokens = pl.tiles && pl.tile.splits == 1 && few_tokens < b.max_query_len ? few_tokens : b.max_query_len;
-    cfg.gridDim = dim3(static_cast<unsigned>(tokens * p.q_heads), static_cast<unsigned>(b.batch));
+    const int64_t longest = pl.tiles && pl.tile.splits == 1 && few_tokens < b.max_query_len ? few_tokens : b.max_query_len;
+    // A row per block of the call where most rows of a longest sequence each would be empty (a prompt of 512 tokens in a
+    // batch of 16: 226 us with a block for every row that the bounds allow).
+    const bool by_token = longest * b.batch > 2 * b.tokens && b.batch <= 1024 && b.tokens * p.q_heads <= 0x7FFFFFFF;
+    const bool many = pl.splits > 8;
+    const int64_t rows = (by_token ? b.tokens : longest) * p.q_heads;
+    cfg.gridDim = dim3(static_cast<unsigned>(many ? rows : div_up(rows, 4)), static_cast<unsigned>(by_token ? 1 : b.batch));
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -676,7 +711,8 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_combine_kernel<D>, p, 8 * pl.nt, 2 * pl.tile.tokens_per_tile * p.group, pl.tile.chunk);
+    e = cudaLaunchKernelEx(&cfg, many ? paged_combine_kernel<D, 4> : paged_combine_kernel<D, 1>, p, 8 * pl.nt,
+                           2 * pl.tile.tokens_per_tile * p.group, pl.tile.chunk, by_token);
   }
   if (e != cudaSuccess) {
     set_error("paged_attention launch failed: %s", cudaGetErrorString(e));
