@@ -85,7 +85,8 @@ def test_bad_batches_are_refused(lib, base, change, words):
     (dict(q_heads=3), b"multiple of the key heads"), (dict(q_heads=0), b"multiple of the key heads"),
     (dict(out_kind=0), b"int8, fp16 or bf16"), (dict(out_kind=4), b"int8, fp16 or bf16"), (dict(q=None), b"null"),
     (dict(out=None), b"null"), (dict(ld_q=250), b"aligned"), (dict(ld_q=128), b"aligned"), (dict(max_kv_len=-1), b"max_kv_len"),
-    (dict(max_kv_len=1 << 20), b"workspace"),
+    (dict(max_kv_len=1 << 20), b"workspace"), (dict(max_kv_len=1 << 30), b"max_kv_len"),
+    (dict(alpha_qk=float("nan")), b"finite"), (dict(alpha_qk=-1e21), b"finite"), (dict(alpha_pv=float("inf")), b"finite"),
 ])
 def test_bad_attention_arguments_are_refused(lib, base, change, words):
     a = dict(q=base, ld_q=256, q_heads=4, max_kv_len=64, out=base, out_kind=1, alpha_qk=1.0, alpha_pv=1.0)
@@ -135,6 +136,9 @@ def test_workspace_query():
     one = f(1, 1, 8, 8, 128, 1, 100000)  # one long sequence: split
     assert one > 0 and one % (8 * (128 * 4 + 8)) == 0
     assert f(1, 1, 8, 8, 128, 5, 100000) == one  # the bound is cut to the tokens
+    # bounds far above the lengths: at most 512 MB
+    for batch, tokens, longest, keys in [(64, 2111, 2048, 131072), (1, 4096, 4096, 1 << 19), (256, 256, 1, 1 << 20), (512, 9000, 64, 1 << 29)]:
+        assert 0 <= f(batch, tokens, 64, 8, 128, longest, keys) <= 512 << 20
 
 
 def test_python_entry_points_refuse_cpu_tensors():

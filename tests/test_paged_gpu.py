@@ -209,6 +209,65 @@ def test_wide_block_table_view(cuda_ops):
     assert_context(out, want, spread, 3)
 
 
+def test_more_sequences_than_the_tile_kernel_takes_at_once(cuda_ops):
+    """600 sequences, two thirds of them with enough new tokens for the tile kernel."""
+    new = [20 + i % 7 if i % 3 else 1 for i in range(600)]
+    keys = [t + (7 * i) % 50 for i, t in enumerate(new)]
+    run_attention(cuda_ops, new, keys, 1, 1, 16, 64, torch.float16, 115)
+
+
+@pytest.mark.parametrize("new,keys", [([1, 5, 2], [40, 300, 1500]), ([30], [64])])
+def test_more_query_heads_than_a_tile_has_rows(cuda_ops, new, keys):
+    run_attention(cuda_ops, new, keys, 160, 1, 16, 64, torch.bfloat16, 116)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 4, 80), (12, 1, 64)])
+def test_prompt_among_decoding_sequences(cuda_ops, heads, kv_heads, dim):
+    """One prompt and many single tokens, all with several splits: both kernels and the joining of both."""
+    new, keys = [1] * 7 + [300] + [1, 0, 3, 1] * 2, [50, 5000, 2900, 1, 4096, 7000, 33, 4000, 6000, 12, 900, 6500, 4, 3, 3, 3333]
+    run_attention(cuda_ops, new, keys, heads, kv_heads, 32, dim, torch.float16, 117)
+
+
+def test_bad_sequence_beside_a_prompt(cuda_ops):
+    """A sequence with bad lengths in such a batch: its rows stay, the others are served."""
+    new, keys = [1, 1, 200] + [1] * 9, [300, 5000, 4200] + [2000 + 300 * i for i in range(9)]
+    b = make_batch(new, keys, 1, 16, 64, 118)
+    q = rand_s8((b["tokens"], 2, 64), 119)
+    want, spread = P.paged_attention(q, *index_args(b), 1e-4, 0.02)
+    b["kv_lens"][1] = 1 << 20
+    g = cuda(b)
+    out = torch.full((b["tokens"], 2, 64), 9.0, dtype=torch.float16, device="cuda")
+    cuda_ops.paged_attention(q.cuda(), *index_args(g), alpha_qk=1e-4, alpha_pv=0.02, max_query_len=200, max_kv_len=5000, out=out)
+    assert cuda_ops.device_status() == 211
+    assert bool((out[1] == 9.0).all())
+    assert_context(out, want, spread, 1)
+    assert_context(out[2:], want[2:], spread[2:], b["tokens"] - 2)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_pages_beyond_four_gigabytes(cuda_ops, new):
+    """Pages whose offset in the pool does not fit 32 bits, appended to and read."""
+    b = make_batch([new, 1], [400, 300], 8, 128, 128, 125)
+    rows = rand_s8((new + 1, 24, 128), 126)
+    kp, vp = b["k_pages"].clone(), b["v_pages"].clone()
+    P.paged_append(rows[:, 8:16], rows[:, 16:], kp, vp, b["block_table"], b["query_starts"], b["kv_lens"])
+    want, spread = P.paged_attention(rows[:, :8], kp, vp, *index_args(b)[2:], 1e-4, 0.02)
+    pages, total = kp.shape[0], 33000  # of 128 KB
+    g = cuda(b)
+    for name in ("k_pages", "v_pages"):
+        far = torch.empty((total, 8, 128, 128), dtype=torch.int8, device="cuda")
+        far[total - pages:] = g[name]
+        g[name] = far
+    used = g["block_table"] >= 0
+    g["block_table"] = torch.where(used, g["block_table"] + (total - pages), g["block_table"])
+    r = rows.cuda()
+    cuda_ops.paged_append(r[:, 8:16], r[:, 16:], *index_args(g))
+    out = cuda_ops.paged_attention(r[:, :8], *index_args(g), alpha_qk=1e-4, alpha_pv=0.02, out_dtype=torch.float16)
+    assert cuda_ops.device_status() == 0
+    assert torch.equal(g["k_pages"][total - pages:].cpu(), kp) and torch.equal(g["v_pages"][total - pages:].cpu(), vp)
+    assert_context(out, want, spread, new + 1)
+
+
 def test_bad_lengths_and_pages_are_reported(cuda_ops):
     """Lengths beyond the bounds or the table, tokens beyond N, pages outside the pool: a status, no fault, and the
     other sequences are served."""
@@ -402,6 +461,34 @@ def test_captured_step_follows_the_lengths(cuda_ops, new):
             assert torch.equal(g["k_pages"].cpu(), kp)
             assert_context(out, want, spread, 2 * new)
     assert C.device_status() == 0
+
+
+def test_captured_mixed_batch_follows_the_lengths(cuda_ops):
+    """Both attention kernels and the join of their splits in one graph; afterwards the lengths move between them."""
+    C = cuda_ops
+    heads, kv_heads, dim, cap, n = 8, 2, 128, 5000, 170
+    b = make_batch([160, 1, 1, 8], [cap] * 4, kv_heads, 64, dim, 411)
+    g = cuda(b)
+    q = rand_s8((n, heads, dim), 412).cuda()
+    out = torch.empty((n, heads, dim), dtype=torch.float16, device="cuda")
+
+    def step():
+        C.paged_attention(q, *index_args(g), alpha_qk=1e-4, alpha_pv=0.02, max_query_len=160, max_kv_len=cap, out=out)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for starts, lens in [([0, 160, 161, 162, 170], [cap] * 4), ([0, 1, 161, 162, 170], [4800, 160, 1, 3000]), ([0, 1, 2, 3, 4], [4999, 1, 700, 64])]:
+        b["query_starts"], b["kv_lens"] = torch.tensor(starts, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32)
+        g["query_starts"].copy_(b["query_starts"])
+        g["kv_lens"].copy_(b["kv_lens"])
+        out.fill_(7.0)
+        graph.replay()
+        assert C.device_status() == 0
+        want, spread = P.paged_attention(q.cpu(), *index_args(b), 1e-4, 0.02)
+        assert_context(out, want, spread, starts[-1])
+        assert bool((out[starts[-1]:] == 7.0).all())
 
 
 def test_calls_on_two_streams_at_once(cuda_ops):

@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "gemm_i8.h"
@@ -574,6 +575,8 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
 constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
 constexpr int MIN_CHUNK = 512, MAX_CHUNK = 2048;  // keys of a split of paged_rows_kernel
+constexpr int64_t MAX_PARTIAL_BYTES = 512ll << 20;
+constexpr int64_t MAX_KEYS = (1 << 30) - 4096;  // a position plus a split stays within 31 bits
 
 // How a call is cut.  Sequences with at most `few` rows per key head are served by paged_rows_kernel, the others by
 // paged_tiles_kernel; a kernel is left out where the bounds show that no sequence needs it.
@@ -600,17 +603,24 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   const int64_t shortest = tokens - (batch - 1) * max_query_len;
   pl.rows = !pl.tiles || shortest * group <= pl.few;
   pl.splits = 1;
+  // Bounds far above the lengths would ask for gigabytes of partial results that nobody writes (64 sequences bound to
+  // 131072 keys with a prompt of 2048 tokens, 64 heads: 4.5 GB): fewer and longer splits there.
+  const int64_t most_splits = MAX_PARTIAL_BYTES / (tokens * group * kv_heads * (head_dim * 4 + 8));
   if (pl.rows) {
     const int64_t most = rows < pl.few ? rows : pl.few;
-    pl.nt = most <= 8 ? 1 : 2;
+    // Beside a prompt the sequences with few rows mostly have a single token: tiles of 8 rows where that is enough for its
+    // heads, 16 otherwise and where every sequence may have more.
+    const int64_t usual = pl.tiles && group <= 8 ? group : most;
+    pl.nt = usual <= 8 ? 1 : 2;
     pl.row_tiles = static_cast<int>(div_up(most, 8 * pl.nt));
     // One CTA per unit where that fills the SMs, in pieces of at most MAX_CHUNK keys (sequences of unequal lengths:
     // 64 contexts of up to 8192 keys took 94 us in pieces of 1024 to 2048 keys, 102 in whole).  Otherwise as many pieces
     // as fill the SMs once (two contexts of 131072 keys: 82 us so, 110 with a third more pieces), of at least MIN_CHUNK
     // keys (one context of 500 keys: 7.6 us in one piece, 8.8 in four).
-    const int64_t units = batch * kv_heads * pl.row_tiles, slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 4);
+    const int64_t units = batch * kv_heads * div_up(usual, 8 * pl.nt), slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 4);
     int64_t chunk = units >= slots ? MAX_CHUNK : round_up(div_up(max_kv_len, slots / units), STEP);
     if (chunk < MIN_CHUNK) chunk = MIN_CHUNK;
+    if (div_up(max_kv_len, chunk) > most_splits) chunk = round_up(div_up(max_kv_len, most_splits > 1 ? most_splits : 1), STEP);
     pl.chunk = static_cast<int>(chunk);
     pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
     // Three warps to a CTA instead of four where the work then runs in fewer rounds, by more than each takes longer:
@@ -637,7 +647,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     const int64_t units = kv_heads * (by_tokens < by_bounds ? by_tokens : by_bounds), tiles = div_up(max_kv_len, 128);
     const double beside = pl.rows ? static_cast<double>((batch - 1) * max_kv_len * kv_heads) * head_dim * 2 / 6.5e6 : 0.0;
     double best = 0;
-    for (int64_t n = 1; n <= 64 && n <= (tiles > 0 ? tiles : 1); ++n) {
+    for (int64_t n = 1; n <= 64 && (n == 1 || (n <= tiles && n <= most_splits)); ++n) {
       const int64_t part = div_up(tiles, n);
       if (n > 1 && div_up(tiles, part) != n) continue;  // the same parts as a smaller n
       const double item = 1.8 * static_cast<double>(part) + 4.0, alone = static_cast<double>(div_up(units * n, PAGED_SMS)) * item;
@@ -745,8 +755,12 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
     set_error("paged_attention: the output must be int8, fp16 or bf16");
     return TI_E_INVALID;
   }
-  if (a.max_kv_len < 0 || a.max_kv_len > 0x7FFFFFFF) {
-    set_error("paged_attention: max_kv_len out of range");
+  if (a.max_kv_len < 0 || a.max_kv_len > MAX_KEYS) {
+    set_error("paged_attention: max_kv_len must be from 0 to %lld (got %lld)", (long long)MAX_KEYS, (long long)a.max_kv_len);
+    return TI_E_INVALID;
+  }
+  if (!(fabsf(a.alpha_qk) <= 1e20f) || !(fabsf(a.alpha_pv) <= 1e20f)) {  // the running maximum starts at -1e30
+    set_error("paged_attention: alpha_qk and alpha_pv must be finite, of at most 1e20");
     return TI_E_INVALID;
   }
   if (b.batch == 0 || b.tokens == 0 || b.max_query_len == 0) return TI_OK;
