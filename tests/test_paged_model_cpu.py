@@ -109,6 +109,49 @@ def test_chunks_and_single_tokens_give_what_one_step_gives(cpu_model):
     assert torch.allclose(torch.cat(parts), whole, rtol=1e-5, atol=1e-5)
 
 
+def test_advanced_steps_and_their_counts(cpu_model):
+    """Steps advanced in place give what new steps give; the cache is told afterwards; what has no page is never 0."""
+    dec = cpu_model.model.decoder
+    x = prompts_of(12)[0]
+    c = dec.new_paged_cache(6)
+    a, b = c.open(), c.open()
+    s = c.step([a, b], [17, 1])
+    assert s.block_table[1, 1] == -1
+    with pytest.raises(ValueError, match="single tokens"):
+        s.advance()
+    c = dec.new_paged_cache(2)
+    whole = dec.forward_paged(x, c, c.step([c.open()], [12]))
+    c = dec.new_paged_cache(2)
+    a = c.open()
+    c.reserve({a: 20})
+    parts = [dec.forward_paged(x[:9], c, c.step([a], [9]))]
+    s = c.step([a], [1])
+    for i in (9, 10, 11):
+        if i > 9:
+            s.advance()
+        parts.append(dec.forward_paged(x[i:i + 1], c, s))
+    assert torch.allclose(torch.cat(parts), whole, rtol=1e-5, atol=1e-5)
+    assert c.length(a) == 10 and s.max_kv_len == 12
+    c.fill(a, 12)
+    assert c.step([a], [1]).positions.tolist() == [12]
+    for bad in (12, 33):
+        with pytest.raises(ValueError, match="filled"):
+            c.fill(a, bad)
+
+
+def test_model_limits_are_refused(cpu_model):
+    dec = cpu_model.model.decoder
+    c = dec.new_paged_cache(8)
+    s = c.step([c.open()], [3])
+    with pytest.raises(ValueError, match="2 tokens given"):
+        dec.forward_paged(torch.tensor([5, 6]), c, s)
+    with pytest.raises(ValueError, match="beyond the model"):
+        dec.forward_paged(torch.full((65,), 5), c, c.step([c.open()], [65]))
+    with pytest.raises(ValueError, match="exceed the model"):
+        cpu_model.generate_paged(prompts_of(60), 6)
+    assert cpu_model.generate_paged(prompts_of(60), 5, use_cuda_graph=False)[0].shape == (65,)
+
+
 def test_generation_agrees_with_teacher_forcing_and_leaves_the_cache(cpu_model):
     prompts = prompts_of(4, 17, 9)
     cache = cpu_model.new_paged_cache(12)

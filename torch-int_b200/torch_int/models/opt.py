@@ -725,10 +725,16 @@ class Int8OPTDecoder(nn.Module):
         and replayed (PagedStep.advance).  The attention does not round its probabilities to int8 (see
         C.paged_attention), so results differ from the static cache's in their last digits."""
         n = tokens.shape[0]
+        if n != step.positions.shape[0]:
+            raise ValueError(f"{n} tokens given, the step brings {step.positions.shape[0]}")
+        if step.longest > self.max_target_positions:
+            raise ValueError(f"position {step.longest - 1} is beyond the model's {self.max_target_positions}")
         hidden = self.embed_tokens(tokens)
         if self.project_in is not None:
             hidden = self.project_in(hidden)
-        hidden = hidden + nn.functional.embedding(step.positions + self.embed_positions.offset, self.embed_positions.weight)
+        # (replays may pass the last position, which only the device sees: the last embedding then, not a bad address)
+        at = (step.positions + self.embed_positions.offset).clamp_(max=self.embed_positions.weight.shape[0] - 1)
+        hidden = hidden + nn.functional.embedding(at, self.embed_positions.weight)
         hidden = hidden.view(1, n, -1)
         residual = hidden.to(self._stream_dtype(hidden)).contiguous()
         first = self.layers[0].self_attn_layer_norm
@@ -1007,6 +1013,8 @@ class Int8OPTForCausalLM(nn.Module):
         seqs = [cache.open() for _ in lens]
         try:
             cache.reserve({s: n + max_new_tokens - 1 for s, n in zip(seqs, lens)})
+            if max(lens) + max_new_tokens - 1 > dec.max_target_positions:
+                raise ValueError(f"{max(lens)} and {max_new_tokens} new tokens exceed the model's {dec.max_target_positions} positions")
             flat = torch.cat([p.reshape(-1) for p in prompts]).to(device)
             nxt = self.forward_paged(flat, cache, cache.step(seqs, lens)).argmax(dim=-1)
             new = [nxt]

@@ -20,10 +20,18 @@ class PagedStep:
     positions: torch.Tensor      # int32 [N], position of each new token
     last: torch.Tensor           # int32 [B], index of each sequence's last new token
     max_query_len: int
-    max_kv_len: int
+    max_kv_len: int              # bound of kv_lens; raise it to the last length before capturing a step
+    longest: int                 # of kv_lens
 
     def advance(self):
-        """The next step of single tokens, on the current stream: every sequence one position further."""
+        """The next step of single tokens, on the current stream: every sequence one position further, into pages that
+        are reserved (PagedInt8KVCache.reserve before the step that is advanced; a sequence without a page for its
+        position is skipped, and the status word says so).  The cache's own lengths do not follow: see
+        PagedInt8KVCache.fill."""
+        if self.max_query_len != 1:
+            raise ValueError(f"only a step of single tokens can be advanced, this one brings up to {self.max_query_len}")
+        self.longest += 1
+        self.max_kv_len = max(self.max_kv_len, self.longest)
         self.kv_lens.add_(1)
         self.positions.add_(1)
 
@@ -91,7 +99,7 @@ class PagedInt8KVCache:
         for s, t, n in zip(seqs, new_tokens, lens):
             starts.append(starts[-1] + t)
             positions.extend(range(n - t, n))
-            table.extend(self._pages[s] + [0] * (width - len(self._pages[s])))
+            table.extend(self._pages[s] + [-1] * (width - len(self._pages[s])))
             self._lengths[s] = n
         b, n = len(seqs), starts[-1]
         flat = torch.tensor(starts + lens + [x - 1 for x in starts[1:]] + positions + table, dtype=torch.int32)
@@ -99,7 +107,14 @@ class PagedInt8KVCache:
             flat = flat.pin_memory().to(self.device, non_blocking=True)
         cuts = [b + 1, b, b, n, b * width]
         starts_t, lens_t, last, pos, tab = torch.split(flat, cuts)
-        return PagedStep(starts_t, lens_t, tab.view(b, width), pos, last, max(new_tokens), max(lens))
+        return PagedStep(starts_t, lens_t, tab.view(b, width), pos, last, max(new_tokens), max(lens), max(lens))
+
+    def fill(self, seq, length):
+        """Counts the positions of `seq` up to `length` as filled: by steps that were advanced on the device."""
+        if not self._lengths[seq] <= length <= len(self._pages[seq]) * self.page_size:
+            raise ValueError(f"sequence {seq} has {self._lengths[seq]} positions and {len(self._pages[seq])} pages of "
+                             f"{self.page_size}, cannot be filled to {length}")
+        self._lengths[seq] = length
 
     def rewind(self, seq, length):
         """Forgets the positions of `seq` from `length` on (rejected drafts); their pages stay with it."""
