@@ -310,7 +310,7 @@ int ti_paged_append(const ti_paged_batch* batch, const ti_paged_append_args* arg
  * Query head h reads key head h / (q_heads / kv_heads).  Unlike ti_attention_prefill_s8 and
  * ti_decode_attention_s8 the probabilities are not rounded to int8.  A token that sees no key (fewer keys than
  * new tokens) gives 0.  q int8, tokens ld_q elements apart; out_kind: 1 fp16, 2 bf16, 3 int8 (sat_rne).
- * max_kv_len bounds kv_lens.  `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
+ * max_kv_len bounds kv_lens (at most 2^30 - 4096); both factors are finite, of at most 1e20.  `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * contents irrelevant, not shared by calls that may overlap on the GPU; NULL where that is 0 (a call that turns out
  * to need one launches nothing and returns TI_E_WORKSPACE). */
 typedef struct ti_paged_attention_args {

