@@ -644,8 +644,8 @@ def _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, tokens, m
         if not (block_table.dtype is query_starts.dtype is kv_lens.dtype is torch.int32
                 and block_table.get_device() == query_starts.get_device() == kv_lens.get_device() == dev):
             raise RuntimeError("block_table, query_starts and kv_lens must be int32 tensors on the cache's device")
-        table = block_table.shape
-        batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+        table, lens = block_table.shape, kv_lens.shape
+        batch = lens[0] if len(lens) == 1 else -1
         if len(table) != 2 or table[0] != batch or query_starts.shape != (batch + 1,):
             raise RuntimeError(f"block_table {tuple(table)}, query_starts {tuple(query_starts.shape)} and kv_lens "
                                f"{tuple(kv_lens.shape)} must be [B, pages], [B + 1] and [B]")
@@ -667,10 +667,14 @@ def _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, tokens, m
 
 def _paged_rows(t, name, tokens, d, dev, dtype):
     """(heads, element stride between the tokens) of `t` [tokens, heads, d], whose heads and columns are packed."""
-    if not (isinstance(t, torch.Tensor) and t.dim() == 3 and t.get_device() == dev and t.dtype is dtype):
+    try:
+        n, h, dd = t.shape
+        token, head, column = t.stride()
+        same = t.dtype is dtype and t.get_device() == dev
+    except (AttributeError, TypeError, ValueError):  # not a tensor, or not of 3 dimensions
+        same = False
+    if not same:
         raise RuntimeError(f"{name} must be a 3-dimensional {dtype} tensor on the cache's device")
-    n, h, dd = t.shape
-    token, head, column = t.stride()
     if n != tokens or dd != d or (d > 1 and column != 1) or (h > 1 and head != d):
         raise RuntimeError(f"{name} must be [{tokens}, heads, {d}] with packed heads, got shape {tuple(t.shape)} "
                            f"and strides {t.stride()}")
@@ -702,9 +706,12 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     pairs are the two halves of those columns, or neighbours with `interleaved`.  max_query_len bounds the new tokens
     of a sequence (default: N).  Returns the rotated int8 queries [N, Hq, D], or None without q.
     Extends torch.cat((past, new)) of torch_int/models/opt.py:113-116."""
-    if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _PAGED_DTYPES:
-        raise RuntimeError("k must be a 3-dimensional float32, float16, bfloat16 or int8 tensor")
-    n, dtype = k.shape[0], k.dtype
+    try:
+        dtype = k.dtype
+        kind = _PAGED_DTYPES[dtype]
+        n, _, _ = k.shape
+    except (AttributeError, TypeError, ValueError, KeyError):
+        raise RuntimeError("k must be a 3-dimensional float32, float16, bfloat16 or int8 tensor") from None
     batch, dev, _, hkv, _, d, _, _ = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens, n, max_query_len)
     hk, ld_k = _paged_rows(k, "k", n, d, dev, dtype)
     hv, ld_v = _paged_rows(v, "v", n, d, dev, dtype)
@@ -723,7 +730,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
         rows, rd = rotary.shape
         rot_ptr = rotary.data_ptr()
     args = _pack_paged_append(q_ptr, k.data_ptr(), v.data_ptr(), ld_q, ld_k, ld_v, hq, rot_ptr, rows, rd, out_ptr,
-                              q_alpha, k_alpha, v_alpha, _PAGED_DTYPES[dtype], 1 if interleaved else 0)
+                              q_alpha, k_alpha, v_alpha, kind, 1 if interleaved else 0)
     _check(_paged_call(_c_paged_append, batch, args, dev))
     return out
 
@@ -738,9 +745,10 @@ def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     what the block table can hold); close bounds cut the work better.  Returns [N, Hq, D]; rows that belong to no
     sequence are left as they were.
     Replaces the attention core of torch_int/models/opt.py:131-181 for sequences of unequal lengths."""
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise RuntimeError("q must be a 3-dimensional int8 tensor")
-    n = q.shape[0]
+    try:
+        n, _, _ = q.shape
+    except (AttributeError, TypeError, ValueError):
+        raise RuntimeError("q must be a 3-dimensional int8 tensor") from None
     batch, dev, b, hkv, page_size, d, width, max_q = _paged_batch(k_pages, v_pages, block_table, query_starts, kv_lens,
                                                                   n, max_query_len)
     hq, ld_q = _paged_rows(q, "q", n, d, dev, torch.int8)
