@@ -196,6 +196,24 @@ def test_strided_queries_and_given_output(cuda_ops):
     assert bool((out[sum(new):] == 7.0).all())
 
 
+def test_the_stride_of_a_single_token_is_not_used(cuda_ops):
+    """One token with 64 heads on one key head (a tile), the distance to a next token given as 7."""
+    b = make_batch([1], [300], 1, 16, 64, 105)
+    q = rand_s8((1, 64, 64), 106)
+    want, spread = P.paged_attention(q, *index_args(b), 1e-4, 0.02)
+    g, x = cuda(b), q.cuda()
+    out = torch.empty((1, 64, 64), dtype=torch.float16, device="cuda")
+    batch = cuda_ops._paged_batch(*index_args(g), 1, 1)[0]
+    args = cuda_ops._pack_paged_attention(x.data_ptr(), 7, 64, 300, out.data_ptr(), 0, 0, 1e-4, 0.02, 1)
+    rc = cuda_ops._c_paged_attention(batch, args, torch.cuda.current_stream().cuda_stream)
+    if rc == -4:
+        ws = torch.empty(cuda_ops._c_paged_workspace(1, 1, 64, 1, 64, 1, 300), dtype=torch.int8, device="cuda")
+        args = cuda_ops._pack_paged_attention(x.data_ptr(), 7, 64, 300, out.data_ptr(), ws.data_ptr(), ws.numel(), 1e-4, 0.02, 1)
+        rc = cuda_ops._c_paged_attention(batch, args, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and cuda_ops.device_status() == 0
+    assert_context(out, want, spread, 1)
+
+
 def test_wide_block_table_view(cuda_ops):
     """A block table that is a view of a wider one (row stride beyond its width)."""
     b = make_batch([1, 2], [50, 200], 2, 16, 64, 111)

@@ -797,7 +797,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   PagedAttnParams p;
   p.view = make_paged_view(b, status);
   p.q = a.q;
-  p.ld_q = a.ld_q;
+  p.ld_q = b.tokens > 1 ? a.ld_q : a.q_heads * b.head_dim;  // (of one token no stride is read, but the tensor map has one)
   p.q_heads = static_cast<int>(a.q_heads);
   p.group = static_cast<int>(group);
   p.max_kv_len = static_cast<int>(a.max_kv_len);
