@@ -5,8 +5,8 @@
 //
 // paged_rows_kernel serves sequences with few query rows per key head (rows = new tokens x group), decode
 // above all: it is bound by the bytes of the cache, 2 * head_dim per key and key head, each read once.
-//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; a warp takes 32 keys at a time, as two groups of
-//     16 (a group lies in one page, in consecutive bytes).
+//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; each of its 4 warps (3 or 8, where make_plan says why)
+//     takes 32 keys at a time, as two groups of 16 (a group lies in one page, in consecutive bytes).
 //   * Scores transposed, S^T = K . Q^T (m16n8k32 s8, keys as rows, queries as the 8 columns), so that a single
 //     query row wastes 7 of 8 columns and not 15 of 16 rows; the context likewise, O^T = V^T . P^T (m16n8k16
 //     fp16).  The columns of a dot product may be taken in any order as long as both operands agree, and so may
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
 
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
 constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
-constexpr int MIN_CHUNK = 512, MAX_CHUNK = 2048;  // keys of a split of paged_rows_kernel
+constexpr int MIN_CHUNK = 256, MAX_CHUNK = 2048;  // keys of a split of paged_rows_kernel
 constexpr int64_t MAX_PARTIAL_BYTES = 512ll << 20;
 constexpr int64_t MAX_KEYS = (1 << 30) - 4096;  // a position plus a split stays within 31 bits
 
@@ -618,17 +618,24 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     // One CTA per unit where that fills the SMs, in pieces of at most MAX_CHUNK keys (sequences of unequal lengths:
     // 64 contexts of up to 8192 keys took 94 us in pieces of 1024 to 2048 keys, 102 in whole).  Otherwise as many pieces
     // as fill the SMs once (two contexts of 131072 keys: 82 us so, 110 with a third more pieces), of at least MIN_CHUNK
-    // keys (one context of 500 keys: 7.6 us in one piece, 8.8 in four).
+    // keys (one context of 2000 keys, 56 heads: 8.1 us in pieces of 288, 9.9 of 512).
     const int64_t units = batch * kv_heads * div_up(usual, 8 * pl.nt), slots = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 4);
     int64_t chunk = units >= slots ? MAX_CHUNK : round_up(div_up(max_kv_len, slots / units), STEP);
     if (chunk < MIN_CHUNK) chunk = MIN_CHUNK;
+    // Small calls are bound by the steps a warp takes one after another: where a CTA per SM leaves it at most two, its eight
+    // warps beat several CTAs of four (16 contexts of 500 keys, 8 key heads: 5.5 us, 8.3 with four warps; 4 of 1000: 5.1 and
+    // 6.8; two steps are better than a join for the narrow heads: one context of 500 keys 3.9 us whole, 4.3 in two parts).
+    const int64_t alone = units <= PAGED_SMS ? div_up(max_kv_len, PAGED_SMS / units) : 513;
+    const bool eight = pl.nt == 1 && !pl.tiles && alone <= 512;
+    if (eight) chunk = alone > 256 || (head_dim < 128 && max_kv_len <= 512) ? 512 : 256;
     if (div_up(max_kv_len, chunk) > most_splits) chunk = round_up(div_up(max_kv_len, most_splits > 1 ? most_splits : 1), STEP);
     pl.chunk = static_cast<int>(chunk);
     pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
     // Three warps to a CTA instead of four where the work then runs in fewer rounds, by more than each takes longer:
     // 8 sequences of 512 keys, 56 heads (448 units; 444 CTAs of four warps at a time, 592 of three): 21.0 -> 17.8 us.
     const int64_t slots3 = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 3);
-    pl.warps = pl.nt == 1 && pl.row_splits == 1 && 4 * div_up(units, slots3) < 3 * div_up(units, slots) ? 3 : 4;
+    const bool three = pl.nt == 1 && pl.row_splits == 1 && 4 * div_up(units, slots3) < 3 * div_up(units, slots);
+    pl.warps = eight ? 8 : three ? 3 : 4;
     // a cluster holds its CTAs until the last one is done: only where all of them run at once
     pl.cluster = pl.row_splits > 1 && pl.row_splits <= MAX_CLUSTER && units * pl.row_splits <= slots;
     if (!pl.cluster) pl.splits = pl.row_splits;
@@ -702,7 +709,8 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
   }
   cudaError_t e = cudaSuccess;
   if (pl.rows)
-    e = pl.warps == 3 ? launch_rows<D, 1, 3>(b, p, pl, stream)
+    e = pl.warps == 3   ? launch_rows<D, 1, 3>(b, p, pl, stream)
+        : pl.warps == 8 ? launch_rows<D, 1, 8>(b, p, pl, stream)
         : pl.nt == 1  ? launch_rows<D, 1, 4>(b, p, pl, stream)
                       : launch_rows<D, 2, 4>(b, p, pl, stream);
   if (e == cudaSuccess && pl.splits > 1) {
