@@ -5,7 +5,7 @@
 //
 // paged_rows_kernel serves sequences with few query rows per key head (rows = new tokens x group), decode
 // above all: it is bound by the bytes of the cache, 2 * head_dim per key and key head, each read once.
-//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; each of its 4 warps (3 or 8, where make_plan says why)
+//   * A CTA owns one key head, 8 * NT query rows and `chunk` keys; each of its 4 warps (3, 6 or 8 where make_plan says why)
 //     takes 32 keys at a time, as two groups of 16 (a group lies in one page, in consecutive bytes).
 //   * Scores transposed, S^T = K . Q^T (m16n8k32 s8, keys as rows, queries as the 8 columns), so that a single
 //     query row wastes 7 of 8 columns and not 15 of 16 rows; the context likewise, O^T = V^T . P^T (m16n8k16
@@ -625,8 +625,16 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     // Small calls are bound by the steps a warp takes one after another: where a CTA per SM leaves it at most two, its eight
     // warps beat several CTAs of four (16 contexts of 500 keys, 8 key heads: 5.5 us, 8.3 with four warps; 4 of 1000: 5.1 and
     // 6.8; two steps are better than a join for the narrow heads: one context of 500 keys 3.9 us whole, 4.3 in two parts).
-    const int64_t alone = units <= PAGED_SMS ? div_up(max_kv_len, PAGED_SMS / units) : 513;
-    const bool eight = pl.nt == 1 && !pl.tiles && alone <= 512;
+    const int64_t alone = div_up(max_kv_len, units <= PAGED_SMS ? PAGED_SMS / units : 1);
+    const bool eight = pl.nt == 1 && !pl.tiles && units <= PAGED_SMS && alone <= 512;
+    // Up to two units per SM: two CTAs of all the warps that fit, each unit in one piece (six of 128-wide heads: 32 contexts
+    // of 1000 keys, 8 key heads, 15.8 -> 14.2 us, of up to 8000 keys 75 -> 61; eight of the others: 8 of 500, 32 x 64,
+    // 6.2 -> 5.3).  The narrow heads also where that takes two rounds: the longest of unequal contexts then ends sooner
+    // (16 of up to 2000, 32 x 80: 23.3 -> 20.6 us; 12 of up to 2000, 32 x 64: 19.2 -> 18.4), which is what equal ones lose
+    // (29.7 -> 32.2; 12.7 both).  Of 128-wide heads equal ones lose more (336 units: 12.7 -> 16.3 us).
+    const int64_t pieces = slots / units;
+    const bool two = pl.nt == 1 && !pl.tiles && (head_dim == 128 ? pieces == 1 && units <= 2 * PAGED_SMS : pieces == 1 || pieces == 2);
+    if (two) chunk = max_kv_len;
     if (eight) chunk = alone > 256 || (head_dim < 128 && max_kv_len <= 512) ? 512 : 256;
     if (div_up(max_kv_len, chunk) > most_splits) chunk = round_up(div_up(max_kv_len, most_splits > 1 ? most_splits : 1), STEP);
     pl.chunk = static_cast<int>(chunk);
@@ -635,7 +643,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     // 8 sequences of 512 keys, 56 heads (448 units; 444 CTAs of four warps at a time, 592 of three): 21.0 -> 17.8 us.
     const int64_t slots3 = PAGED_SMS * rows_ctas_per_sm(head_dim, pl.nt, 3);
     const bool three = pl.nt == 1 && pl.row_splits == 1 && 4 * div_up(units, slots3) < 3 * div_up(units, slots);
-    pl.warps = eight ? 8 : three ? 3 : 4;
+    pl.warps = eight ? 8 : two ? (head_dim == 128 ? 6 : 8) : three ? 3 : 4;
     // a cluster holds its CTAs until the last one is done: only where all of them run at once
     pl.cluster = pl.row_splits > 1 && pl.row_splits <= MAX_CLUSTER && units * pl.row_splits <= slots;
     if (!pl.cluster) pl.splits = pl.row_splits;
@@ -710,9 +718,10 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
   cudaError_t e = cudaSuccess;
   if (pl.rows)
     e = pl.warps == 3   ? launch_rows<D, 1, 3>(b, p, pl, stream)
+        : pl.warps == 6 ? launch_rows<D, 1, D == 128 ? 6 : 8>(b, p, pl, stream)
         : pl.warps == 8 ? launch_rows<D, 1, 8>(b, p, pl, stream)
-        : pl.nt == 1  ? launch_rows<D, 1, 4>(b, p, pl, stream)
-                      : launch_rows<D, 2, 4>(b, p, pl, stream);
+        : pl.nt == 1    ? launch_rows<D, 1, 4>(b, p, pl, stream)
+                        : launch_rows<D, 2, 4>(b, p, pl, stream);
   if (e == cudaSuccess && pl.splits > 1) {
     cudaLaunchConfig_t cfg = {};
     // only the rows of few-row sequences have partial results where the tile kernel does not split
