@@ -227,6 +227,24 @@ def test_wide_block_table_view(cuda_ops):
     assert_context(out, want, spread, 3)
 
 
+@pytest.mark.parametrize("dim,batch,heads,kv_heads,keys", [
+    (128, 8, 56, 56, 90),     # 448 units: three warps
+    (64, 20, 32, 32, 70),     # 640
+    (128, 32, 16, 8, 300),    # two CTAs of six warps per SM
+    (64, 8, 32, 32, 200),     # of eight
+    (80, 16, 32, 32, 300),    # of eight, two rounds
+    (128, 16, 32, 8, 500),    # a CTA of eight warps per SM
+    (128, 4, 32, 8, 1000),    # four of them in a cluster
+    (80, 1, 16, 2, 9000),     # many, joined through the workspace
+    (128, 6, 56, 56, 200),    # 336: four warps
+    (64, 5, 64, 64, 900),     # pieces of 256 and more, clusters of four warps
+])
+def test_ways_of_cutting_a_decode_step(cuda_ops, dim, batch, heads, kv_heads, keys):
+    """Single tokens, contexts of unequal lengths up to `keys`, one of them a single key and one of the whole length."""
+    lens = [1 + (i * 7919) % keys for i in range(batch - 1)] + [keys]
+    run_attention(cuda_ops, [1] * batch, lens, heads, kv_heads, 16, dim, torch.float16, 113)
+
+
 def test_more_sequences_than_the_tile_kernel_takes_at_once(cuda_ops):
     """600 sequences, two thirds of them with enough new tokens for the tile kernel."""
     new = [20 + i % 7 if i % 3 else 1 for i in range(600)]
