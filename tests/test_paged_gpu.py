@@ -238,11 +238,22 @@ def test_wide_block_table_view(cuda_ops):
     (80, 1, 16, 2, 9000),     # many, joined through the workspace
     (128, 6, 56, 56, 200),    # 336: four warps
     (64, 5, 64, 64, 900),     # pieces of 256 and more, clusters of four warps
+    (128, 2, 32, 8, 2000),    # clusters of eight
 ])
 def test_ways_of_cutting_a_decode_step(cuda_ops, dim, batch, heads, kv_heads, keys):
     """Single tokens, contexts of unequal lengths up to `keys`, one of them a single key and one of the whole length."""
     lens = [1 + (i * 7919) % keys for i in range(batch - 1)] + [keys]
     run_attention(cuda_ops, [1] * batch, lens, heads, kv_heads, 16, dim, torch.float16, 113)
+
+
+@pytest.mark.parametrize("dim,batch,new,heads,kv_heads,keys", [
+    (128, 4, 8, 32, 8, 700), (64, 1, 24, 16, 16, 1000), (80, 2, 5, 32, 8, 500), (128, 16, 5, 32, 8, 400), (64, 3, 33, 4, 4, 300),
+    (128, 1, 5, 32, 8, 2000),
+])
+def test_drafts_of_shared_key_heads(cuda_ops, dim, batch, new, heads, kv_heads, keys):
+    """9 to 32 rows per key head (tiles of 16), and 33."""
+    lens = [max(new, 1 + (i * 7919) % keys) for i in range(batch - 1)] + [keys]
+    run_attention(cuda_ops, [new - (i % 3) for i in range(batch)], lens, heads, kv_heads, 16, dim, torch.bfloat16, 114)
 
 
 def test_more_sequences_than_the_tile_kernel_takes_at_once(cuda_ops):

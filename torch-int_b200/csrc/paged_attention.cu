@@ -575,7 +575,11 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
 }
 
 constexpr int TILE_ROWS = 128;  // rows of a row tile of paged_tiles_kernel
-constexpr int FEW_ROWS = 16;    // rows up to which a sequence is served by paged_rows_kernel
+// Rows up to which a sequence is served by paged_rows_kernel, in tiles of 16 that each read the keys.  16 sequences of 2000
+// keys, 32 query heads on 8 of 128: 8 new tokens (32 rows) 27 us so and 51 by paged_tiles_kernel; 12 (48 rows) 45 both;
+// 48 rows of 32 key heads 144 and 106.
+// Beside longer sequences half as many: 16 decoding sequences and a prompt take 82 us so, 88 with the empty tiles of 32 rows.
+constexpr int FEW_ROWS = 32, FEW_BESIDE = 16;
 constexpr int MIN_CHUNK = 256, MAX_CHUNK = 2048;  // keys of a split of paged_rows_kernel
 constexpr int64_t MAX_PARTIAL_BYTES = 512ll << 20;
 constexpr int64_t MAX_KEYS = (1 << 30) - 4096;  // a position plus a split stays within 31 bits
@@ -601,6 +605,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
   const int64_t rows = max_query_len * group;
   pl.few = group > TILE_ROWS ? 0x7FFFFFFF : FEW_ROWS;
   pl.tiles = rows > pl.few;
+  if (pl.tiles) pl.few = FEW_BESIDE;
   // the shortest sequence brings at least the tokens that the others cannot hold
   const int64_t shortest = tokens - (batch - 1) * max_query_len;
   pl.rows = !pl.tiles || shortest * group <= pl.few;
@@ -625,8 +630,12 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     // Small calls are bound by the steps a warp takes one after another: where a CTA per SM leaves it at most two, its eight
     // warps beat several CTAs of four (16 contexts of 500 keys, 8 key heads: 5.5 us, 8.3 with four warps; 4 of 1000: 5.1 and
     // 6.8; two steps are better than a join for the narrow heads: one context of 500 keys 3.9 us whole, 4.3 in two parts).
+    // But a cluster of eight such CTAs takes eight SMs of one GPC, and few of those are free at a time (two contexts of 2000
+    // keys, 8 key heads: 9.4 us, 6.6 with four warps): more than four only where they are half the SMs at most.
     const int64_t alone = div_up(max_kv_len, units <= PAGED_SMS ? PAGED_SMS / units : 1);
-    const bool eight = pl.nt == 1 && !pl.tiles && units <= PAGED_SMS && alone <= 512;
+    const int64_t chunk8 = alone > 256 || (head_dim < 128 && max_kv_len <= 512) ? 512 : 256, parts8 = div_up(max_kv_len, chunk8);
+    const bool eight = !pl.tiles && units <= PAGED_SMS && alone <= 512 &&
+                       (parts8 <= 4 || parts8 > MAX_CLUSTER || units * parts8 <= PAGED_SMS / 2);
     // Up to two units per SM: two CTAs of all the warps that fit, each unit in one piece (six of 128-wide heads: 32 contexts
     // of 1000 keys, 8 key heads, 15.8 -> 14.2 us, of up to 8000 keys 75 -> 61; eight of the others: 8 of 500, 32 x 64,
     // 6.2 -> 5.3).  The narrow heads also where that takes two rounds: the longest of unequal contexts then ends sooner
@@ -635,7 +644,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     const int64_t pieces = slots / units;
     const bool two = pl.nt == 1 && !pl.tiles && (head_dim == 128 ? pieces == 1 && units <= 2 * PAGED_SMS : pieces == 1 || pieces == 2);
     if (two) chunk = max_kv_len;
-    if (eight) chunk = alone > 256 || (head_dim < 128 && max_kv_len <= 512) ? 512 : 256;
+    if (eight) chunk = chunk8;
     if (div_up(max_kv_len, chunk) > most_splits) chunk = round_up(div_up(max_kv_len, most_splits > 1 ? most_splits : 1), STEP);
     pl.chunk = static_cast<int>(chunk);
     pl.row_splits = static_cast<int>(max_kv_len > chunk ? div_up(max_kv_len, chunk) : 1);
@@ -719,7 +728,7 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const Plan& pl, cudaSt
   if (pl.rows)
     e = pl.warps == 3   ? launch_rows<D, 1, 3>(b, p, pl, stream)
         : pl.warps == 6 ? launch_rows<D, 1, D == 128 ? 6 : 8>(b, p, pl, stream)
-        : pl.warps == 8 ? launch_rows<D, 1, 8>(b, p, pl, stream)
+        : pl.warps == 8 ? (pl.nt == 1 ? launch_rows<D, 1, 8>(b, p, pl, stream) : launch_rows<D, 2, 8>(b, p, pl, stream))
         : pl.nt == 1    ? launch_rows<D, 1, 4>(b, p, pl, stream)
                         : launch_rows<D, 2, 4>(b, p, pl, stream);
   if (e == cudaSuccess && pl.splits > 1) {
