@@ -674,6 +674,7 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     const double beside = pl.rows ? static_cast<double>((batch - 1) * max_kv_len * kv_heads) * head_dim * 2 / 6.5e6 : 0.0;
     double best = 0;
     for (int64_t n = 1; n <= 64 && (n == 1 || (n <= tiles && n <= most_splits)); ++n) {
+      if (n > 1 && units * (n - 1) >= 4 * PAGED_SMS) break;  // four rounds and more: finer parts have nothing to fill
       const int64_t part = div_up(tiles, n);
       if (n > 1 && div_up(tiles, part) != n) continue;  // the same parts as a smaller n
       const double item = 1.8 * static_cast<double>(part) + 4.0, alone = static_cast<double>(div_up(units * n, PAGED_SMS)) * item;
@@ -689,6 +690,10 @@ Plan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, i
     if (pl.tile.splits > pl.splits) pl.splits = pl.tile.splits;
   }
   return pl;
+}
+
+int64_t partial_bytes(const Plan& pl, int64_t tokens, int64_t q_heads, int64_t head_dim) {
+  return pl.splits == 1 ? 0 : tokens * q_heads * pl.splits * (head_dim * 4 + 8);
 }
 
 template <int D, int NT, int WARPS>
@@ -766,7 +771,7 @@ int64_t paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q
   if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_query_len <= 0 || max_kv_len <= 0) return 0;
   if (max_query_len > tokens) max_query_len = tokens;
   const Plan pl = make_plan(batch, tokens, q_heads / kv_heads, kv_heads, static_cast<int>(head_dim), max_query_len, max_kv_len);
-  return pl.splits == 1 ? 0 : tokens * q_heads * pl.splits * (head_dim * 4 + 8);
+  return partial_bytes(pl, tokens, q_heads, head_dim);
 }
 
 int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t stream) {
@@ -808,8 +813,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
               (long long)b.max_query_len);
     return TI_E_INVALID;
   }
-  const int64_t need = paged_attention_workspace_bytes(b.batch, b.tokens, a.q_heads, b.kv_heads, b.head_dim,
-                                                       b.max_query_len, a.max_kv_len);
+  const int64_t need = partial_bytes(pl, b.tokens, a.q_heads, b.head_dim);
   if (need > a.workspace_bytes || (need > 0 && (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15) != 0))) {
     set_error("paged_attention: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
               (long long)a.workspace_bytes);
