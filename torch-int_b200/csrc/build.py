@@ -13,7 +13,8 @@ OUT_DIR = os.path.join(os.path.dirname(HERE), "torch_int", "lib")
 OUT = os.path.join(OUT_DIR, "libtorch_int_b200.so")
 SOURCES = ["gemm_i8_sm100.cu", "norm_quant.cu", "decode_attention.cu", "attention_prefill_sm100.cu",
            "paged_append.cu", "paged_attention.cu", "paged_attention_sm100.cu", "abi.cu"]
-HEADERS = ["gemm_i8.h", "norm_quant.h", "attention_prefill.h", "paged.h", "paged_device.cuh", "paged_attention.cuh", "sm100_ptx.cuh", "grid_dependency.cuh",
+HEADERS = ["gemm_i8.h", "norm_quant.h", "attention_prefill.h", "paged.h", "paged_plan.h", "paged_device.cuh", "paged_attention.cuh",
+           "sm100_ptx.cuh", "grid_dependency.cuh",
            os.path.join("..", "..", "include", "torch_int_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -8,6 +8,7 @@
 #include <atomic>
 
 #include "paged_device.cuh"
+#include "paged_plan.h"
 
 namespace ti {
 
@@ -31,8 +32,6 @@ struct PagedAttnParams {
   float2* part_ml;    // [tokens * q_heads][max_splits]: maximum (log2 domain) and sum
 };
 
-constexpr int PAGED_SMS = 148;
-
 // Runs a kernel's set-up (function attributes) the first time it is launched on a device: a call of its own costs
 // about as much as a launch.
 class PagedOncePerDevice {
@@ -51,13 +50,6 @@ class PagedOncePerDevice {
   std::atomic<unsigned long long> done_{0};
 };
 
-// How the tile kernel (paged_attention_sm100.cu) cuts the work.
-struct PagedTilePlan {
-  int tokens_per_tile;  // of 128 rows: 128 / group
-  int pairs;            // pairs of row tiles of the largest sequence
-  int chunk;            // keys of a split, a multiple of 128
-  int splits;
-};
 int launch_paged_tiles(const PagedBatch& b, const PagedAttnParams& p, const PagedTilePlan& plan, cudaStream_t stream);
 
 struct PagedSplits {
