@@ -1,0 +1,68 @@
+"""How paged_attention cuts a call (csrc/paged_plan.h), compiled by itself for the host and swept over sizes and bounds:
+every launch that a plan leads to has blocks, and every kernel of it has rows to serve."""
+import ctypes
+import itertools
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "torch-int_b200", "csrc")
+FIELDS = ("rows tiles few nt warps row_tiles chunk row_splits cluster tokens_per_tile pairs tile_chunk tile_splits splits "
+          "join_blocks bytes").split()
+WRAPPER = """
+#include "paged_plan.h"
+using namespace ti;
+extern "C" void plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int head_dim, int64_t max_query_len,
+                     int64_t max_kv_len, int64_t* o) {
+  const PagedPlan p = make_plan(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len);
+  const int64_t join = p.splits > 1 ? plan_join(p, batch, tokens, group * kv_heads, group, max_query_len).blocks : -1;
+  const int64_t v[] = {p.rows, p.tiles, p.few, p.nt, p.warps, p.row_tiles, p.chunk, p.row_splits, p.cluster, p.tile.tokens_per_tile,
+                       p.tile.pairs, p.tile.chunk, p.tile.splits, p.splits, join, partial_bytes(p, tokens, group * kv_heads, head_dim)};
+  for (unsigned i = 0; i < sizeof(v) / sizeof(v[0]); ++i) o[i] = v[i];
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(WRAPPER)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", CSRC, "-o", str(d / "plan.so"), str(d / "plan.cpp")])
+    fn = ctypes.CDLL(str(d / "plan.so")).plan
+    i64 = ctypes.c_int64
+    fn.argtypes = [i64, i64, i64, i64, ctypes.c_int, i64, i64, ctypes.POINTER(i64)]
+    fn.restype = None
+
+    def call(*sizes):
+        out = (i64 * len(FIELDS))()
+        fn(*sizes, out)
+        return dict(zip(FIELDS, out))
+    return call
+
+
+def calls(max_kv_lens):
+    """(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len): single tokens, drafts, prompts, and one prompt
+    among single tokens."""
+    for batch, group, kv_heads, dim, keys in itertools.product((1, 2, 8, 16, 33, 64, 300, 600), (1, 3, 8, 16, 17, 32, 40, 71, 128, 129),
+                                                               (1, 2, 8, 40), (64, 128), max_kv_lens):
+        for new in (1, 5, 100, 512, 2048):
+            yield batch, batch * new, group, kv_heads, dim, new, keys
+            if new > 1:
+                yield batch, batch - 1 + new, group, kv_heads, dim, new, keys
+
+
+def test_every_launch_has_blocks_and_every_kernel_has_rows(plan):
+    for sizes in calls((1, 16, 300, 2000, 4000, 8000, 131072)):
+        p = plan(*sizes)
+        group, new = sizes[2], sizes[5]
+        assert p["rows"] or p["tiles"], sizes
+        if p["splits"] > 1:
+            assert 0 < p["join_blocks"] <= 0x7FFFFFFF, (sizes, p)
+        if p["rows"]:
+            assert group <= p["few"], (sizes, p)  # a sequence with a single token has `group` rows
+            assert p["row_tiles"] >= 1 and p["row_splits"] >= 1, (sizes, p)
+        if p["tiles"]:
+            assert p["tokens_per_tile"] >= 1 and p["pairs"] >= 1 and p["tile_splits"] >= 1, (sizes, p)
+            assert group * new > p["few"], (sizes, p)
+        assert p["bytes"] <= 512 << 20, (sizes, p)

@@ -56,7 +56,8 @@ inline PagedPlan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t
   if (pl.tiles) pl.few = FEW_BESIDE;
   // the shortest sequence brings at least the tokens that the others cannot hold
   const int64_t shortest = tokens - (batch - 1) * max_query_len;
-  pl.rows = !pl.tiles || shortest * group <= pl.few;
+  // (beside a prompt, tokens with more heads on a key head than `few` are the tile kernel's: no rows kernel is needed)
+  pl.rows = !pl.tiles || (group <= pl.few && shortest * group <= pl.few);
   pl.splits = 1;
   // Bounds far above the lengths would ask for gigabytes of partial results that nobody writes (64 sequences bound to
   // 131072 keys with a prompt of 2048 tokens, 64 heads: 4.5 GB): fewer and longer splits there.
