@@ -17,3 +17,11 @@ def test_prompt_among_tokens_of_many_heads_per_key_head(cuda_ops, heads, kv_head
     new = [1] * (batch - 1) + [prompt]
     keys = [1 + (i * 7919) % longest for i in range(batch - 2)] + [longest, max(prompt, longest // 2)]
     run_attention(cuda_ops, new, keys, heads, kv_heads, 16, dim, torch.float16, 803)
+
+
+@pytest.mark.parametrize("new,batch,heads,kv_heads,dim", [(1, 300, 1, 1, 64), (1, 32, 32, 8, 128), (1, 32, 32, 8, 64), (3, 3, 4, 2, 80),
+                                                          (1, 8, 56, 56, 128), (40, 2, 8, 2, 128)])
+def test_a_step_without_any_key_gives_zeros(cuda_ops, new, batch, heads, kv_heads, dim):
+    """Every sequence holds no key, and the bound says so: max_kv_len = 0."""
+    out, _ = run_attention(cuda_ops, [new] * batch, [0] * batch, heads, kv_heads, 16, dim, torch.float16, 811)
+    assert bool((out == 0).all())

@@ -66,3 +66,14 @@ def test_every_launch_has_blocks_and_every_kernel_has_rows(plan):
             assert p["tokens_per_tile"] >= 1 and p["pairs"] >= 1 and p["tile_splits"] >= 1, (sizes, p)
             assert group * new > p["few"], (sizes, p)
         assert p["bytes"] <= 512 << 20, (sizes, p)
+
+
+def test_the_pieces_cover_the_keys(plan):
+    """Bounds from no key at all on (a step whose sequences hold none gives zeros)."""
+    for sizes in calls((0, 1, 31, 300, 4000, 131072)):
+        p = plan(*sizes)
+        keys = sizes[6]
+        if p["rows"]:
+            assert p["chunk"] > 0 and p["chunk"] % 32 == 0 and p["chunk"] * p["row_splits"] >= keys, (sizes, p)
+        if p["tiles"]:
+            assert p["tile_chunk"] > 0 and p["tile_chunk"] % 128 == 0 and p["tile_chunk"] * p["tile_splits"] >= keys, (sizes, p)

@@ -23,7 +23,7 @@ struct PagedAttnParams {
   void* out;
   int out_kind;       // 1 fp16, 2 bf16, 3 int8
   int row_tiles;      // of the largest sequence
-  int chunk;          // keys of a split, a multiple of 16
+  int chunk;          // keys of a split, a multiple of 32
   int max_splits;     // stride of the partial results
   int cluster;        // the splits of the rows kernel are a cluster and need no partial results
   int rows_below;     // sequences with at most this many rows belong to the rows kernel, the others to the tile kernel

@@ -92,7 +92,7 @@ inline PagedPlan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t
     // (29.7 -> 32.2; 12.7 both).  Of 128-wide heads equal ones lose more (336 units: 12.7 -> 16.3 us).
     const int64_t pieces = slots / units;
     const bool two = pl.nt == 1 && !pl.tiles && (head_dim == 128 ? pieces == 1 && units <= 2 * PAGED_SMS : pieces == 1 || pieces == 2);
-    if (two) chunk = max_kv_len;
+    if (two) chunk = round_up(max_kv_len > 0 ? max_kv_len : 1, STEP);
     if (eight) chunk = chunk8;
     if (div_up(max_kv_len, chunk) > most_splits) chunk = round_up(div_up(max_kv_len, most_splits > 1 ? most_splits : 1), STEP);
     pl.chunk = static_cast<int>(chunk);
