@@ -25,3 +25,21 @@ def test_a_step_without_any_key_gives_zeros(cuda_ops, new, batch, heads, kv_head
     """Every sequence holds no key, and the bound says so: max_kv_len = 0."""
     out, _ = run_attention(cuda_ops, [new] * batch, [0] * batch, heads, kv_heads, 16, dim, torch.float16, 811)
     assert bool((out == 0).all())
+
+
+def test_lengths_written_by_the_kernel_before(cuda_ops):
+    """Lengths and starts that change on the stream right before each call, joined through the workspace."""
+    b = make_batch([1] * 3, [9000] * 3, 2, 16, 128, 821)
+    q = rand_s8((3, 16, 128), 822)
+    lens = [torch.tensor(x, dtype=torch.int32) for x in ([9000, 30, 4000], [2, 9000, 8999], [5000, 7000, 1], [900, 1800, 2700])]
+    want = [P.paged_attention(q, *index_args(b)[:4], x, 2e-4, 0.02) for x in lens]
+    g, gq, glens = cuda(b), q.cuda(), [x.cuda() for x in lens]
+    outs = [torch.empty((3, 16, 128), dtype=torch.float16, device="cuda") for _ in range(200)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        g["kv_lens"].copy_(glens[i % 4])
+        cuda_ops.paged_attention(gq, *index_args(g), alpha_qk=2e-4, alpha_pv=0.02, max_query_len=1, max_kv_len=9000, out=out)
+    assert cuda_ops.device_status() == 0
+    for i in range(4):
+        assert_context(outs[i], *want[i], 3)
+        assert all(torch.equal(outs[i], x) for x in outs[i::4])

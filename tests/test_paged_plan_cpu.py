@@ -77,3 +77,17 @@ def test_the_pieces_cover_the_keys(plan):
             assert p["chunk"] > 0 and p["chunk"] % 32 == 0 and p["chunk"] * p["row_splits"] >= keys, (sizes, p)
         if p["tiles"]:
             assert p["tile_chunk"] > 0 and p["tile_chunk"] % 128 == 0 and p["tile_chunk"] * p["tile_splits"] >= keys, (sizes, p)
+
+
+def test_kernels_read_the_index_arrays_behind_their_wait():
+    """A kernel that is launched as a programmatic dependent may start before the writer of query_starts, kv_lens or the
+    block table is done; only griddepcontrol.wait orders its reads behind those writes."""
+    for name, kernels in (("paged_attention.cu", ("paged_rows_kernel", "paged_combine_kernel")), ("paged_append.cu", ("paged_append_kernel",))):
+        with open(os.path.join(CSRC, name)) as f:
+            source = f.read()
+        for kernel in kernels:
+            start = source.index("__global__", source.rindex("template", 0, source.index(kernel + "(const")))
+            body = source[start:source.index("\n}\n", start)]
+            wait = body.index("grid_dep_wait()")
+            for read in ("query_starts[", "kv_lens[", "paged_sequence(", "paged_page(", "rows_of_a_cta<"):
+                assert read not in body[:wait], (kernel, read)

@@ -479,7 +479,9 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
   const unsigned row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x;
   const int head = row % p.q_heads;
   int t = row / p.q_heads, b = blockIdx.y;
-  // (The index arrays are read before the wait: no kernel that lets its dependents start early writes them.)
+  // The lengths too are read behind the wait: the rows kernel lets this one start before it has itself waited for whoever
+  // wrote them.
+  grid_dep_wait();
   if (by_token) {
     b = -1;
     for (int i = lane; i < v.batch; i += 32) {
@@ -489,9 +491,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
     b = __reduce_max_sync(0xffffffffu, b);
   }
   PagedSeq s;
-  const bool ok = b >= 0 && paged_sequence(v, b, p.max_kv_len, &s);
-  grid_dep_wait();
-  if (!ok) return;
+  if (b < 0 || !paged_sequence(v, b, p.max_kv_len, &s)) return;
   if (by_token) t -= s.q0;
   if (t >= s.T) return;
   // the row tile this row belonged to decides how many keys, hence splits, were visited
