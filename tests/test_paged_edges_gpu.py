@@ -43,3 +43,37 @@ def test_lengths_written_by_the_kernel_before(cuda_ops):
     for i in range(4):
         assert_context(outs[i], *want[i], 3)
         assert all(torch.equal(outs[i], x) for x in outs[i::4])
+
+
+@pytest.mark.parametrize("new,keys", [(1, 300), (20, 300), (150, 300), (150, 3000), (300, 300)])
+@pytest.mark.parametrize("alpha", [2.7, -2.7, 4.0, 16.0, -16.0, 1000.0, 1e20])
+def test_steep_scores(cuda_ops, new, keys, alpha):
+    """Factors at which one unit of q . k decides, for one token and for prompts.  q . k is within 64, so to the bound of
+    assert_context comes the rounding of a score of up to 64 * alpha powers of e to fp32, twice: 2 s 2^-23 of a weight.  From
+    alpha = 16 on only the keys with the largest q . k count (the others have 2^-23 of their weight or less, 3000 keys 2^-11,
+    and that rounding of it): their scores are equal numbers, so the term falls away."""
+    dim = 64
+    b = make_batch([new, 1], [keys, 40], 2, 16, dim, 831)
+    b["k_pages"] = rand_s8(tuple(b["k_pages"].shape), 832, -1, 1)
+    q = rand_s8((new + 1, 4, dim), 833, -1, 1)
+    want, spread = P.paged_attention(q, *index_args(b), alpha, 0.02)
+    out = cuda_ops.paged_attention(q.cuda(), *index_args(cuda(b)), alpha_qk=alpha, alpha_pv=0.02, out_dtype=torch.float16)
+    assert cuda_ops.device_status() == 0 and bool(out.isfinite().all())
+    term = 2 * 64 * abs(alpha) * 1.4427 * 2.0 ** -23 if abs(alpha) < 16 else 0.0
+    tol = spread * (2.0 ** -11 + 2.0 ** -15 + term) + want.abs() * 2.0 ** -11 * 1.001 + 2.0 ** -25
+    err = (out.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("new,keys", [(1, 300), (150, 300), (150, 3000)])
+@pytest.mark.parametrize("alpha", [2.7, -2.7, 16.0, 1e20])
+def test_steep_scores_far_from_zero(cuda_ops, new, keys, alpha):
+    """The largest q . k there is, the same for every key: every context is the mean of the values it sees."""
+    dim = 128
+    b = make_batch([new], [keys], 1, 16, dim, 841)
+    b["k_pages"].fill_(-128)
+    q = torch.full((new, 2, dim), -128, dtype=torch.int8)
+    want, spread = P.paged_attention(q, *index_args(b), 0.0, 0.02)
+    out = cuda_ops.paged_attention(q.cuda(), *index_args(cuda(b)), alpha_qk=alpha, alpha_pv=0.02, out_dtype=torch.float16)
+    assert cuda_ops.device_status() == 0
+    assert_context(out, want, spread, new)

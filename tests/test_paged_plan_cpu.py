@@ -14,8 +14,8 @@ WRAPPER = """
 #include "paged_plan.h"
 using namespace ti;
 extern "C" void plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int head_dim, int64_t max_query_len,
-                     int64_t max_kv_len, int64_t* o) {
-  const PagedPlan p = make_plan(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len);
+                     int64_t max_kv_len, float scale_log2, int64_t* o) {
+  const PagedPlan p = make_plan_for_scale(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len, scale_log2);
   const int64_t join = p.splits > 1 ? plan_join(p, batch, tokens, group * kv_heads, group, max_query_len).blocks : -1;
   const int64_t v[] = {p.rows, p.tiles, p.few, p.nt, p.warps, p.row_tiles, p.chunk, p.row_splits, p.cluster, p.tile.tokens_per_tile,
                        p.tile.pairs, p.tile.chunk, p.tile.splits, p.splits, join, partial_bytes(p, tokens, group * kv_heads, head_dim)};
@@ -31,12 +31,12 @@ def plan(tmp_path_factory):
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", CSRC, "-o", str(d / "plan.so"), str(d / "plan.cpp")])
     fn = ctypes.CDLL(str(d / "plan.so")).plan
     i64 = ctypes.c_int64
-    fn.argtypes = [i64, i64, i64, i64, ctypes.c_int, i64, i64, ctypes.POINTER(i64)]
+    fn.argtypes = [i64, i64, i64, i64, ctypes.c_int, i64, i64, ctypes.c_float, ctypes.POINTER(i64)]
     fn.restype = None
 
-    def call(*sizes):
+    def call(*sizes, scale_log2=1e-3):
         out = (i64 * len(FIELDS))()
-        fn(*sizes, out)
+        fn(*sizes, scale_log2, out)
         return dict(zip(FIELDS, out))
     return call
 
@@ -91,3 +91,17 @@ def test_kernels_read_the_index_arrays_behind_their_wait():
             wait = body.index("grid_dep_wait()")
             for read in ("query_starts[", "kv_lens[", "paged_sequence(", "paged_page(", "rows_of_a_cta<"):
                 assert read not in body[:wait], (kernel, read)
+
+
+def test_steep_scores_are_the_rows_kernels(plan):
+    """Factors that the tile kernel's fp32 offset cannot carry: its sequences go to the rows kernel, without more workspace
+    than ti_paged_attention_workspace_bytes, which does not know the factor, gives for the sizes."""
+    for sizes in calls((0, 300, 4000, 131072)):
+        flat = plan(*sizes)
+        assert plan(*sizes, scale_log2=4.0) == plan(*sizes, scale_log2=-4.0) == flat
+        for scale in (4.1, -23.0, 1.4e20):
+            p = plan(*sizes, scale_log2=scale)
+            assert p["rows"] and not p["tiles"] and p["bytes"] <= flat["bytes"], (sizes, scale, p)
+            assert p["chunk"] > 0 and p["chunk"] * p["row_splits"] >= sizes[6], (sizes, scale, p)
+            assert p["row_tiles"] * 8 * p["nt"] >= sizes[2] * sizes[5], (sizes, scale, p)
+            assert p["splits"] == 1 or 0 < p["join_blocks"] <= 0x7FFFFFFF, (sizes, scale, p)

@@ -672,7 +672,9 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
     return TI_E_INVALID;
   }
   const int64_t group = a.q_heads / b.kv_heads;
-  const PagedPlan pl = make_plan(b.batch, b.tokens, group, b.kv_heads, static_cast<int>(b.head_dim), b.max_query_len, a.max_kv_len);
+  const float scale_log2 = static_cast<float>(static_cast<double>(a.alpha_qk) * 1.4426950408889634);
+  const PagedPlan pl = make_plan_for_scale(b.batch, b.tokens, group, b.kv_heads, static_cast<int>(b.head_dim), b.max_query_len,
+                                           a.max_kv_len, scale_log2);
   if (b.batch * static_cast<int64_t>(pl.row_tiles) > 65535 || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
     set_error("paged_attention: batch %lld x %lld new tokens is too large for one call", (long long)b.batch,
               (long long)b.max_query_len);
@@ -696,7 +698,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   p.q_heads = static_cast<int>(a.q_heads);
   p.group = static_cast<int>(group);
   p.max_kv_len = static_cast<int>(a.max_kv_len);
-  p.scale_log2 = static_cast<float>(static_cast<double>(a.alpha_qk) * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.alpha_pv = a.alpha_pv;
   p.out = a.out;
   p.out_kind = a.out_kind;

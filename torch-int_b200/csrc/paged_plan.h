@@ -47,11 +47,12 @@ struct PagedPlan {
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t div_up(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
+// `rows_only`, if not 0: every sequence is served by paged_rows_kernel, in at most so many splits.
 inline PagedPlan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int head_dim, int64_t max_query_len,
-                           int64_t max_kv_len) {
+                           int64_t max_kv_len, int64_t rows_only = 0) {
   PagedPlan pl = {};
   const int64_t rows = max_query_len * group;
-  pl.few = group > TILE_ROWS ? 0x7FFFFFFF : FEW_ROWS;
+  pl.few = group > TILE_ROWS || rows_only > 0 ? 0x7FFFFFFF : FEW_ROWS;
   pl.tiles = rows > pl.few;
   if (pl.tiles) pl.few = FEW_BESIDE;
   // the shortest sequence brings at least the tokens that the others cannot hold
@@ -61,7 +62,8 @@ inline PagedPlan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t
   pl.splits = 1;
   // Bounds far above the lengths would ask for gigabytes of partial results that nobody writes (64 sequences bound to
   // 131072 keys with a prompt of 2048 tokens, 64 heads: 4.5 GB): fewer and longer splits there.
-  const int64_t most_splits = MAX_PARTIAL_BYTES / (tokens * group * kv_heads * (head_dim * 4 + 8));
+  int64_t most_splits = MAX_PARTIAL_BYTES / (tokens * group * kv_heads * (head_dim * 4 + 8));
+  if (rows_only > 0 && rows_only < most_splits) most_splits = rows_only;
   if (pl.rows) {
     const int64_t most = rows < pl.few ? rows : pl.few;
     // Beside a prompt the sequences with few rows mostly have a single token: tiles of 8 rows where that is enough for its
@@ -143,6 +145,19 @@ inline PagedPlan make_plan(int64_t batch, int64_t tokens, int64_t group, int64_t
 
 inline int64_t partial_bytes(const PagedPlan& pl, int64_t tokens, int64_t q_heads, int64_t head_dim) {
   return pl.splits == 1 ? 0 : tokens * q_heads * pl.splits * (head_dim * 4 + 8);
+}
+
+// paged_tiles_kernel keeps its scores relative to an fp32 number of about |scale_log2| * 1.5 * 2^23, whose spacing moves
+// the largest exponent, meant to be 7, by up to |scale_log2|: at 4 it stays within 3 .. 11 of the 15 that fp16 holds, at
+// 12 it would pass them.  Steeper factors (a unit of q . k is then worth more than 2^4) are left to paged_rows_kernel,
+// whose exponents are exact; it needs no larger workspace for them than the sizes alone ask for.
+constexpr float MAX_TILE_SCALE = 4.f;
+
+inline PagedPlan make_plan_for_scale(int64_t batch, int64_t tokens, int64_t group, int64_t kv_heads, int head_dim,
+                                     int64_t max_query_len, int64_t max_kv_len, float scale_log2) {
+  const PagedPlan pl = make_plan(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len);
+  if (!pl.tiles || (scale_log2 >= -MAX_TILE_SCALE && scale_log2 <= MAX_TILE_SCALE)) return pl;
+  return make_plan(batch, tokens, group, kv_heads, head_dim, max_query_len, max_kv_len, pl.splits);
 }
 
 // The launch of paged_combine_kernel, which joins the partial results of a plan with splits > 1.
