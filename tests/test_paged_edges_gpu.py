@@ -77,3 +77,26 @@ def test_steep_scores_far_from_zero(cuda_ops, new, keys, alpha):
     out = cuda_ops.paged_attention(q.cuda(), *index_args(cuda(b)), alpha_qk=alpha, alpha_pv=0.02, out_dtype=torch.float16)
     assert cuda_ops.device_status() == 0
     assert_context(out, want, spread, new)
+
+
+@pytest.mark.parametrize("alpha,unit", [(5.6, -115), (5.63, -128), (5.67, -128), (5.7, -122)])
+@pytest.mark.parametrize("new,batch,heads", [(1, 64, 8), (5, 64, 32), (150, 2, 8)])
+def test_scores_that_rise_by_just_what_the_maximum_may_lag_behind(cuda_ops, alpha, unit, new, batch, heads):
+    """Scores near 2^24 are 2 apart in fp32.  Here later keys are 8 above the first ones: not more than a running maximum
+    may lag behind, but one more than that once 7 minus the maximum is rounded.  All values are equal, and so is each
+    context, whatever the weights."""
+    dim, kv_heads, keys = 128, 8, 1024
+    b = make_batch([new] * batch, [keys] * batch, kv_heads, 64, dim, 851)
+    b["k_pages"].fill_(-128)
+    row = torch.arange(64)
+    for s in range(batch):
+        for i in range(keys // 64):  # 256 keys with `unit` in the last column, 256 with one more
+            b["k_pages"][b["block_table"][s, i], :, row, dim - 1] = unit + (i // 4) % 2
+    b["v_pages"].fill_(50)
+    q = torch.full((new * batch, heads, dim), -128, dtype=torch.int8)
+    q[..., dim - 1] = 1
+    out = cuda_ops.paged_attention(q.cuda(), *index_args(cuda(b)), alpha_qk=alpha, alpha_pv=0.02, max_query_len=new, max_kv_len=keys,
+                                   out_dtype=torch.float16)
+    assert cuda_ops.device_status() == 0
+    want = torch.full(out.shape, 50 * 0.02, dtype=torch.float64)
+    assert_context(out, want, want, new * batch)

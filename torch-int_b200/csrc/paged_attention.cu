@@ -17,8 +17,8 @@
 //     by the latency of its own instructions, not by the depth of the queue (2, 3 and 4 groups in flight: the same):
 //     hence 32 keys a step, whose two halves overlap.
 //   * int8 values become fp16 exactly (byte + 1152 as the low bits of 1024.., minus 1152).
-//   * Running maximum in the log2 domain per warp, raised only when a score exceeds it by more than 8 (a vote,
-//     no reduction, in the common case); probabilities are 2^(s - max + 7) <= 2^15, split into two fp16 numbers
+//   * Running maximum in the log2 domain per warp, raised only when an exponent s + (7 - max) passes 15 (a vote,
+//     no reduction, in the common case); probabilities are 2^(s + (7 - max)) <= 2^15, split into two fp16 numbers
 //     (p = hi + lo, 22 bits) whose products are summed in fp32: the tensor cores have room for the second
 //     product because the loop waits for memory.
 // Measured: 64 contexts of 8192 keys, 8 key heads x 128, 166 us (6.5 TB/s); 128 of 2048 82 us; 2 of 131072 76 us; 8 of 640,
@@ -283,7 +283,7 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
           mma_s8(acc, fa, qf[n].w[2 * k], qf[n].w[2 * k + 1]);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sc[u][n][c] = static_cast<float>(acc[c]) * p.scale_log2;
+        for (int c = 0; c < 4; ++c) sc[u][n][c] = __fmul_rn(static_cast<float>(acc[c]), p.scale_log2);  // (not contracted: `raise` relies on it)
       }
     }
     if (key + STEP - 1 > lim_min) {
@@ -302,7 +302,7 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         top[n][c] = fmaxf(fmaxf(sc[0][n][c], sc[0][n][c + 2]), fmaxf(sc[1][n][c], sc[1][n][c + 2]));
-        raise |= top[n][c] > m[n][c] + 8.f;
+        raise |= top[n][c] + (7.f - m[n][c]) > 15.f;  // the sum that the exponents below are, rounded alike
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
