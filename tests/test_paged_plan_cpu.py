@@ -105,3 +105,20 @@ def test_steep_scores_are_the_rows_kernels(plan):
             assert p["chunk"] > 0 and p["chunk"] * p["row_splits"] >= sizes[6], (sizes, scale, p)
             assert p["row_tiles"] * 8 * p["nt"] >= sizes[2] * sizes[5], (sizes, scale, p)
             assert p["splits"] == 1 or 0 < p["join_blocks"] <= 0x7FFFFFFF, (sizes, scale, p)
+
+
+def test_workspace_query_of_sizes_that_no_call_accepts():
+    """Sizes that ti_paged_attention refuses need no workspace, and no arithmetic on them may end the process."""
+    from torch_int import _CUDA as C
+    ask = C._c_paged_workspace
+    good = dict(batch=2, tokens=2, q_heads=64, kv_heads=8, head_dim=128, max_query_len=1, max_kv_len=131072)
+    assert ask(*good.values()) > 0
+    huge = (1 << 62, (1 << 63) - 1, -(1 << 63), -1, 0)
+    for field in good:
+        for bad in huge + {"head_dim": (-2, 72), "q_heads": (63, 65536), "kv_heads": (65536, 3), "batch": (65536,),
+                           "tokens": (1 << 31,), "max_kv_len": (1 << 30,)}.get(field, ()):
+            if field == "max_query_len" and bad > 0:
+                continue  # a bound: cut to the tokens
+            assert ask(*{**good, field: bad}.values()) == 0, (field, bad)
+    for sizes in itertools.product((1 << 62, 1 << 32), repeat=7):
+        assert ask(*sizes) == 0

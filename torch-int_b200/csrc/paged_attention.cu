@@ -633,7 +633,11 @@ int launch(const PagedBatch& b, const PagedAttnParams& p, const PagedPlan& pl, c
 
 int64_t paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
                                         int64_t head_dim, int64_t max_query_len, int64_t max_kv_len) {
-  if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_query_len <= 0 || max_kv_len <= 0) return 0;
+  // none for calls without tokens or keys, and for sizes that paged_attention refuses
+  if (batch <= 0 || batch > 65535 || tokens <= 0 || tokens > 0x7FFFFFFF || kv_heads <= 0 || q_heads <= 0 || q_heads > 65535 ||
+      q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 80 && head_dim != 128) || max_query_len <= 0 ||
+      max_kv_len <= 0 || max_kv_len > MAX_KEYS)
+    return 0;
   if (max_query_len > tokens) max_query_len = tokens;
   const PagedPlan pl = make_plan(batch, tokens, q_heads / kv_heads, kv_heads, static_cast<int>(head_dim), max_query_len, max_kv_len);
   return partial_bytes(pl, tokens, q_heads, head_dim);
