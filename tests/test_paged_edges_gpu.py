@@ -100,3 +100,27 @@ def test_scores_that_rise_by_just_what_the_maximum_may_lag_behind(cuda_ops, alph
     assert cuda_ops.device_status() == 0
     want = torch.full(out.shape, 50 * 0.02, dtype=torch.float64)
     assert_context(out, want, want, new * batch)
+
+
+@pytest.mark.parametrize("bound", [1 << 31, 1 << 32, (1 << 32) + 1, (1 << 63) - 1])
+def test_a_bound_of_the_new_tokens_beyond_32_bits(cuda_ops, bound):
+    """max_query_len of the C entry points is 64 bits wide: any value from the longest sequence's on serves the batch."""
+    C = cuda_ops
+    new, keys = [3, 1], [40, 33]
+    b = make_batch(new, keys, 2, 16, 64, 861)
+    rows = rand_s8((4, 6, 64), 862)
+    kp, vp = b["k_pages"].clone(), b["v_pages"].clone()
+    P.paged_append(rows[:, 2:4], rows[:, 4:], kp, vp, *index_args(b)[2:])
+    want, spread = P.paged_attention(rows[:, :2], kp, vp, *index_args(b)[2:], 1e-4, 0.02)
+    g, r = cuda(b), rows.cuda()
+    out = torch.empty((4, 2, 64), dtype=torch.float16, device="cuda")
+    pages, table = b["k_pages"].shape[0], b["block_table"].shape[1]
+    batch = C._pack_paged_batch(*(t.data_ptr() for t in index_args(g)), pages, 2, 16, 64, table, table, 2, 4, bound)
+    stream = torch.cuda.current_stream().cuda_stream
+    base = r.data_ptr()
+    append = C._pack_paged_append(0, base + 128, base + 256, 0, 384, 384, 0, 0, 0, 0, 0, 1.0, 1.0, 1.0, 3, 0)
+    assert C._c_paged_append(batch, append, stream) == 0
+    assert C._c_paged_attention(batch, C._pack_paged_attention(base, 384, 2, 40, out.data_ptr(), 0, 0, 1e-4, 0.02, 1), stream) == 0
+    assert C.device_status() == 0
+    assert torch.equal(g["k_pages"].cpu(), kp) and torch.equal(g["v_pages"].cpu(), vp)
+    assert_context(out, want, spread, 4)

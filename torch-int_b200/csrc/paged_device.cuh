@@ -35,7 +35,7 @@ inline PagedView make_paged_view(const PagedBatch& b, int* status) {
   while ((1ll << v.page_shift) < b.page_size) ++v.page_shift;
   v.batch = static_cast<int>(b.batch);
   v.tokens = static_cast<int>(b.tokens);
-  v.max_query_len = static_cast<int>(b.max_query_len);
+  v.max_query_len = static_cast<int>(b.max_query_len < b.tokens ? b.max_query_len : b.tokens);
   v.status = status;
   return v;
 }
