@@ -124,3 +124,31 @@ def test_a_bound_of_the_new_tokens_beyond_32_bits(cuda_ops, bound):
     assert C.device_status() == 0
     assert torch.equal(g["k_pages"].cpu(), kp) and torch.equal(g["v_pages"].cpu(), vp)
     assert_context(out, want, spread, 4)
+
+
+@pytest.mark.parametrize("batch,new,heads,alpha", [(33000, 2, 10, 1e-4), (70, 1900, 8, 16.0)])
+def test_more_row_tiles_than_a_grid_is_high(cuda_ops, batch, new, heads, alpha):
+    """33000 sequences with two row tiles each, and 70 whose bound of 1900 tokens of 8 heads asks for 950 each (a steep factor:
+    the rows kernel's), the first and the last of them longer than the rest.  The sequences share their pages."""
+    keys = 40
+    short = 2
+    b = make_batch([0], [keys], 1, 16, 64, 871)
+    b["k_pages"] = rand_s8(tuple(b["k_pages"].shape), 872, -1, 1)
+    news = [new if i in (0, batch - 1) else short for i in range(batch)]
+    starts = torch.tensor([0] + news, dtype=torch.int32).cumsum(0).to(torch.int32)
+    lens = torch.full((batch,), keys, dtype=torch.int32)
+    lens[-1] = keys - 3
+    n = int(starts[-1])
+    q = rand_s8((short, heads, 64), 873, -1, 1).repeat(-(-n // short), 1, 1)[:n].contiguous()
+    g = cuda(b)
+    out = cuda_ops.paged_attention(q.cuda(), g["k_pages"], g["v_pages"], g["block_table"].expand(batch, -1).contiguous(), starts.cuda(),
+                                   lens.cuda(), alpha_qk=alpha, alpha_pv=0.02, max_query_len=new, max_kv_len=keys, out_dtype=torch.float16)
+    assert cuda_ops.device_status() == 0
+    seen = {}
+    for i in {0, 1, batch // 2, batch - 2, batch - 1}:
+        at, t = int(starts[i]), news[i]
+        want, spread = P.paged_attention(q[at:at + t], *index_args(b)[:3], [0, t], [int(lens[i])], alpha, 0.02)
+        assert_context(out[at:at + t], want, spread, t)
+        seen[i] = out[at:at + t]
+    middle = out[int(starts[1]):int(starts[batch - 1])].view(batch - 2, short, heads, 64)
+    assert bool((middle == seen[1]).all())

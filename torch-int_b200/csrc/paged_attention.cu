@@ -198,7 +198,7 @@ __device__ __forceinline__ void rows_of_a_cta(const PagedAttnParams& p) {
   float* s_join = reinterpret_cast<float*>(smem + SM::JOINED);
   const PagedView& v = p.view;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, a = lane & 3;
-  const int b = blockIdx.z / p.row_tiles, rt = blockIdx.z % p.row_tiles, h = blockIdx.y, split = blockIdx.x;
+  const int tile = p.first_tile + blockIdx.z, b = tile / p.row_tiles, rt = tile % p.row_tiles, h = blockIdx.y, split = blockIdx.x;
   // the first entries of the block table are loaded beside the lengths, not behind them (one latency less)
   const unsigned first_page = static_cast<unsigned>(split * p.chunk + (warp + WARPS * (lane >> 1)) * STEP + (lane & 1) * 16) >> v.page_shift;
   const int first_entry = first_page < static_cast<unsigned>(v.table_width) ? v.table[b * v.table_ld + first_page] : -1;
@@ -568,18 +568,18 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnParam
   if (mine) paged_store4(p, at * D + d, x, sum > 0.f ? p.alpha_pv / sum : 0.f);
 }
 
+constexpr int64_t MAX_GRID_Z = 65535;
+
 template <int D, int NT, int WARPS>
-cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const PagedPlan& pl, cudaStream_t stream) {
+cudaError_t launch_rows(const PagedBatch& b, PagedAttnParams p, const PagedPlan& pl, cudaStream_t stream) {
   auto kernel = paged_rows_kernel<D, NT, WARPS>;
   constexpr int smem = RowsSmem<D, NT, WARPS>::BYTES;
   static PagedOncePerDevice once;
-  const cudaError_t e = once.run([kernel] {
+  cudaError_t e = once.run([kernel] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
-                     static_cast<unsigned>(b.batch * pl.row_tiles));
   cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -592,7 +592,14 @@ cudaError_t launch_rows(const PagedBatch& b, const PagedAttnParams& p, const Pag
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pl.cluster ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  const int64_t tiles = b.batch * pl.row_tiles;
+  for (int64_t first = 0; first < tiles && e == cudaSuccess; first += MAX_GRID_Z) {
+    p.first_tile = static_cast<int>(first);
+    cfg.gridDim = dim3(static_cast<unsigned>(pl.row_splits), static_cast<unsigned>(b.kv_heads),
+                       static_cast<unsigned>(tiles - first < MAX_GRID_Z ? tiles - first : MAX_GRID_Z));
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+  }
+  return e;
 }
 
 template <int D>
@@ -679,7 +686,7 @@ int paged_attention(const PagedBatch& b0, const PagedAttention& a, cudaStream_t 
   const float scale_log2 = static_cast<float>(static_cast<double>(a.alpha_qk) * 1.4426950408889634);
   const PagedPlan pl = make_plan_for_scale(b.batch, b.tokens, group, b.kv_heads, static_cast<int>(b.head_dim), b.max_query_len,
                                            a.max_kv_len, scale_log2);
-  if (b.batch * static_cast<int64_t>(pl.row_tiles) > 65535 || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
+  if (b.batch * static_cast<int64_t>(pl.row_tiles) > 0x7FFFFFFF - MAX_GRID_Z || b.max_query_len * a.q_heads > 0x7FFFFFFF) {
     set_error("paged_attention: batch %lld x %lld new tokens is too large for one call", (long long)b.batch,
               (long long)b.max_query_len);
     return TI_E_INVALID;

@@ -23,6 +23,7 @@ struct PagedAttnParams {
   void* out;
   int out_kind;       // 1 fp16, 2 bf16, 3 int8
   int row_tiles;      // of the largest sequence
+  int first_tile;     // of the launch, counted over the sequences
   int chunk;          // keys of a split, a multiple of 32
   int max_splits;     // stride of the partial results
   int cluster;        // the splits of the rows kernel are a cluster and need no partial results
