@@ -74,3 +74,20 @@ def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, alp
             y = (p @ val[:, None]).permute(2, 0, 1, 3).reshape(t, hq, d)
             dst[q0:q0 + t] = y * (alpha_pv if dst is ctx else abs(alpha_pv))
     return ctx, spread
+
+
+def model_attention(sd, prefix, hidden_int8, mask, num_heads, past=None, trace=None):
+    """attention() of opt_model.py as the paged model path computes it: probabilities kept in 64 bits, not rounded to units
+    of 1/127, so the scale of pv_bmm, which counts those units, is taken 127 times; one rounding of the context to int8."""
+    from . import opt_model as OM
+    bsz, tgt, e = hidden_int8.shape
+    d = e // num_heads
+    x2d = hidden_int8.reshape(-1, e)
+    q, k, v = (OM._linear_s8(sd, f"{prefix}.{n}", x2d).view(bsz, tgt, num_heads, d).transpose(1, 2) for n in ("q_proj", "k_proj", "v_proj"))
+    if past is not None:
+        k, v = torch.cat([past[0], k], dim=2), torch.cat([past[1], v], dim=2)
+    scores = (q.double() @ k.double().transpose(2, 3)) * OM._f(sd, prefix + ".qk_bmm.a")
+    p = torch.softmax(scores.masked_fill(mask < 0, float("-inf")), dim=-1)
+    ctx = (127.0 * OM._f(sd, prefix + ".pv_bmm.a") * (p @ v.double())).round().clamp(-128, 127).to(torch.int8)
+    ctx = ctx.transpose(1, 2).reshape(bsz * tgt, e).contiguous()
+    return OM._linear_f32(sd, prefix + ".out_proj", ctx).view(bsz, tgt, e), (k, v)
