@@ -1027,13 +1027,14 @@ class Int8OPTForCausalLM(nn.Module):
                 left -= 1
             if left > 0 and use_cuda_graph:
                 static = nxt.clone()
-                graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph):
-                    step.advance()
-                    static.copy_(self.forward_paged(static, cache, step).argmax(dim=-1))
-                for _ in range(left):
-                    graph.replay()
-                    new.append(static.clone())
+                with torch.cuda.device(device):  # a capture records the current device's streams alone
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        step.advance()
+                        static.copy_(self.forward_paged(static, cache, step).argmax(dim=-1))
+                    for _ in range(left):
+                        graph.replay()
+                        new.append(static.clone())
             else:
                 for _ in range(left):
                     step.advance()
