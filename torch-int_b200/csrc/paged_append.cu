@@ -259,9 +259,10 @@ int check_paged_batch(const PagedBatch& b, const char* name) {
     set_error("%s: page_size must be 16, 32, 64, 128 or 256 (got %lld)", name, (long long)b.page_size);
     return TI_E_INVALID;
   }
+  const int64_t most_pages = 0x7FFFFFFF / b.page_size;
   if (b.kv_heads <= 0 || b.kv_heads > 65535 || b.batch < 0 || b.batch > 65535 || b.tokens < 0 || b.tokens > 0x7FFFFFFF ||
-      b.max_query_len < 0 || b.num_pages <= 0 || b.num_pages * b.page_size > 0x7FFFFFFF || b.table_width <= 0 ||
-      b.table_width * b.page_size > 0x7FFFFFFF || b.table_ld < b.table_width) {
+      b.max_query_len < 0 || b.num_pages <= 0 || b.num_pages > most_pages || b.table_width <= 0 || b.table_width > most_pages ||
+      b.table_ld < b.table_width) {
     set_error("%s: sizes out of range (batch %lld, tokens %lld, kv_heads %lld, %lld pages of %lld, block table %lld wide)",
               name, (long long)b.batch, (long long)b.tokens, (long long)b.kv_heads, (long long)b.num_pages,
               (long long)b.page_size, (long long)b.table_width);
