@@ -270,7 +270,10 @@ int ti_attention_prefill_s8(const int8_t* q, int64_t ld_q, int64_t q_batch_strid
  *
  * A sequence whose lengths disagree with `tokens`, the bounds or the width of the block table is skipped (nothing
  * of it is read or written) and sets the status word of ti_device_status to 211; a block table entry outside the
- * pool sets it to 212 (its tokens are not stored; an attention that meets it reads page 0 instead). */
+ * pool sets it to 212 (its tokens are not stored; an attention that meets it reads page 0 instead).
+ *
+ * At most 65535 sequences, key heads and query heads, 2^31 - 1 tokens, positions of the pool and positions a row of the block
+ * table spans.  Two sequences may share pages that neither appends to in this call. */
 typedef struct ti_paged_batch {
   int8_t* k_pages;
   int8_t* v_pages;
@@ -289,7 +292,9 @@ typedef struct ti_paged_batch {
  * Pair i is columns (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`.  rotary NULL: no rotation.
  * dtype of q, k and v: 0 fp32, 1 fp16, 2 bf16, 3 int8.  Token t of k starts at k + t * ld_k elements, heads and
  * columns packed (q and v likewise; column blocks of a fused projection can be passed).  q NULL: no queries;
- * otherwise q_out int8 [tokens, q_heads, head_dim].  rotary_dim a multiple of 16; all rows 16-byte aligned. */
+ * otherwise q_out int8 [tokens, q_heads, head_dim].  rotary_dim a multiple of 16; all rows 16-byte aligned.  A token that is not
+ * stored (a skipped sequence, a page outside the pool, a position the table does not reach: 211) leaves its row of q_out as it
+ * was, and so do tokens of no sequence. */
 typedef struct ti_paged_append_args {
   const void* q;
   const void* k;
@@ -310,7 +315,12 @@ int ti_paged_append(const ti_paged_batch* batch, const ti_paged_append_args* arg
  * Query head h reads key head h / (q_heads / kv_heads).  Unlike ti_attention_prefill_s8 and
  * ti_decode_attention_s8 the probabilities are not rounded to int8.  A token that sees no key (fewer keys than
  * new tokens) gives 0.  q int8, tokens ld_q elements apart; out_kind: 1 fp16, 2 bf16, 3 int8 (sat_rne).
- * max_kv_len bounds kv_lens (at most 2^30 - 4096); both factors are finite, of at most 1e20.  `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
+ * Probabilities of a sequence with more than 32 (beside a longer one 16) query rows per key head - new tokens x query heads that
+ * share it, of which there are 128 at most - are rounded to fp16 (2^-11) for the products with v, all others to 2^-21; sums
+ * are fp32.
+ * max_kv_len bounds kv_lens (from 0 to 2^30 - 4096); both factors are finite, of at most 1e20 (prompts with alpha_qk beyond 2.77
+ * are served by the kernel for few rows, five times slower).  max_query_len x q_heads is at most 2^31 - 1.
+ * `workspace`: at least ti_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * contents irrelevant, not shared by calls that may overlap on the GPU; NULL where that is 0 (a call that turns out
  * to need one launches nothing and returns TI_E_WORKSPACE). */
 typedef struct ti_paged_attention_args {
@@ -324,7 +334,7 @@ typedef struct ti_paged_attention_args {
 } ti_paged_attention_args;
 int ti_paged_attention(const ti_paged_batch* batch, const ti_paged_attention_args* args, void* stream);
 
-/* Bytes of workspace ti_paged_attention needs for these sizes (0: none). */
+/* Bytes of workspace ti_paged_attention needs for these sizes (0: none, or sizes that it refuses). */
 int64_t ti_paged_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
                                            int64_t head_dim, int64_t max_query_len, int64_t max_kv_len);
 

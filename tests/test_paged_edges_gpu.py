@@ -152,3 +152,21 @@ def test_more_row_tiles_than_a_grid_is_high(cuda_ops, batch, new, heads, alpha):
         seen[i] = out[at:at + t]
     middle = out[int(starts[1]):int(starts[batch - 1])].view(batch - 2, short, heads, 64)
     assert bool((middle == seen[1]).all())
+
+
+def test_queries_of_tokens_that_are_not_stored_keep_their_rows(cuda_ops):
+    """A sequence with bad lengths, a page outside the pool and tokens of no sequence: their rows of q_out stay."""
+    C = cuda_ops
+    b = make_batch([2, 1, 2], [20, 9, 40], 2, 16, 64, 881, extra_tokens=2)
+    b["kv_lens"][1] = -1
+    b["block_table"][2, 2] = -1  # positions 38 and 39
+    rows = rand_s8((7, 6, 64), 882)
+    g, r = cuda(b), rows.cuda()
+    q_out = torch.full((7, 2, 64), 77, dtype=torch.int8, device="cuda")
+    pages, table = b["k_pages"].shape[0], b["block_table"].shape[1]
+    batch = C._pack_paged_batch(*(t.data_ptr() for t in index_args(g)), pages, 2, 16, 64, table, table, 3, 7, 2)
+    base = r.data_ptr()
+    append = C._pack_paged_append(base, base + 128, base + 256, 384, 384, 384, 2, 0, 0, 0, q_out.data_ptr(), 1.0, 1.0, 1.0, 3, 0)
+    assert C._c_paged_append(batch, append, torch.cuda.current_stream().cuda_stream) == 0
+    assert C.device_status() in (211, 212)
+    assert torch.equal(q_out[:2].cpu(), rows[:2, :2]) and bool((q_out[2:] == 77).all())

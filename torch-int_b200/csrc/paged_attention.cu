@@ -21,8 +21,8 @@
 //     no reduction, in the common case); probabilities are 2^(s + (7 - max)) <= 2^15, split into two fp16 numbers
 //     (p = hi + lo, 22 bits) whose products are summed in fp32: the tensor cores have room for the second
 //     product because the loop waits for memory.
-// Measured: 64 contexts of 8192 keys, 8 key heads x 128, 166 us (6.5 TB/s); 128 of 2048 82 us; 2 of 131072 76 us; 8 of 640,
-// 56 heads, 15.5 us (one round of CTAs: latency).
+// Measured: 64 contexts of 8192 keys, 8 key heads x 128, 168 us (6.4 TB/s); 128 of 2048 83 us; 2 of 131072 88 us; 8 of 640,
+// 56 heads, 14.7 us (one round of CTAs: latency).
 // The keys are split over CTAs.  Up to MAX_CLUSTER splits are a cluster, whose CTAs join their partial results
 // through distributed shared memory: one launch, no workspace.  More splits write them in fp32 to a workspace and
 // paged_combine_kernel joins them.  Both in a fixed order, without atomics: results do not depend on timing.

@@ -4,7 +4,7 @@
 // A CTA owns one key head of one sequence and two tiles of 128 query rows (a row is a token and one of the query
 // heads that share the key head) and walks over 128-key tiles:
 //   S = Q . K^T      tcgen05 kind::i8, Q and K as TMA stores them (128-byte swizzle), int32 in TMEM;
-//   p = 2^(s - off)  one thread per row, S read from TMEM once; p is written back over S as fp16;
+//   p = 2^(s - off)  two threads per row, S read from TMEM once; p goes as fp16 to columns of its own (S is free by then);
 //   O += P . V       tcgen05 kind::f16, A = P from TMEM, B = V from shared memory, fp32 in TMEM.
 // V arrives as int8 rows (keys) and one warpgroup turns it into fp16, exactly, in the layout in which the head
 // dimension is the contiguous one: no transpose, and 256 query rows share one conversion.
@@ -27,9 +27,9 @@
 // context is still being written.
 // The score is formed without a conversion instruction: the bits of 1.5 * 2^23 + acc are acc + constant (|acc| <=
 // 2^21), and one fused multiply-add with off = c * (1.5 * 2^23 + max) - 7 gives the exponent; whatever off was
-// rounded to, it is the same for the whole row and cancels in the division by the sum.  off is raised only when an
-// exponent passes 15 (p <= 2^15 fits fp16 and, against the maximum's 2^7 or more, keeps weights down to 2^-31);
-// then O in TMEM is rescaled by the row's thread.  p is rounded to fp16 (2^-11) for the product, the row sum uses
+// rounded to, it is the same for the whole row and cancels in the division by the sum (as long as the rounding leaves the
+// exponents within fp16: MAX_TILE_SCALE in paged_plan.h).  off is raised only when an exponent passes 15 (p <= 2^15 fits fp16 and, against the maximum's 2^7 or more, keeps weights down to 2^-31);
+// then O in TMEM is rescaled by the row's threads.  p is rounded to fp16 (2^-11) for the product, the row sum uses
 // it unrounded in fp32.  Every wait is bounded (2 s) and reports through the status word.
 // Measured: 2048 tokens behind 14336, 32 query heads on 8 of 128: 446 us, 1155 TFLOP/s, 3400 clocks per 256 x 128 scores
 // (the exponentials and their conversion keep their pipe busy for 2300 of them, issue for 2500); 8 prompts of 512, 56

@@ -704,7 +704,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     block_table int32 [B, >= pages of the longest]: its pages in order.  int8 = sat_rne(alpha * x) after rotating
     the first columns of q and k by `rotary`, fp32 [positions, rotary_dim] (torch_int.functional.paged.rotary_table):
     pairs are the two halves of those columns, or neighbours with `interleaved`.  max_query_len bounds the new tokens
-    of a sequence (default: N).  Returns the rotated int8 queries [N, Hq, D], or None without q.
+    of a sequence (default: N).  Returns the rotated int8 queries [N, Hq, D], or None without q; rows of tokens that were not
+    stored (see device_status) or belong to no sequence hold nothing.
     Extends torch.cat((past, new)) of torch_int/models/opt.py:113-116."""
     try:
         dtype = k.dtype
@@ -741,9 +742,10 @@ def paged_attention(q, k_pages, v_pages, block_table, query_starts, kv_lens, *, 
     token per sequence to whole prompts.  q int8 [N, Hq, D] (heads and columns packed, any token stride), Hq a
     multiple of the cache's heads; cache and index tensors as in paged_append, the new tokens already stored.
     ctx = alpha_pv * softmax(alpha_qk * q . k) . v, rounded once to `out_dtype` (int8, float16 or bfloat16) or to
-    `out`'s; a token that sees no key gives 0.  max_query_len and max_kv_len bound the lengths (default: N and
-    what the block table can hold); close bounds cut the work better.  Returns [N, Hq, D]; rows that belong to no
-    sequence are left as they were.
+    `out`'s; a token that sees no key gives 0.  Probabilities are rounded to fp16 for sequences with more than 32 (beside a
+    longer one 16) new tokens x heads per key head, to 2^-21 otherwise.  max_query_len and max_kv_len bound the lengths
+    (default: N and what the block table can hold); close bounds cut the work better.  Returns [N, Hq, D]; rows that
+    belong to no sequence are left as they were.
     Replaces the attention core of torch_int/models/opt.py:131-181 for sequences of unequal lengths."""
     try:
         n, _, _ = q.shape
